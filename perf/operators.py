@@ -18,6 +18,7 @@ Layout of one layer (n_pages pages of P tokens, Hk kv heads, head_dim D):
 import math
 import random
 
+import numpy as np
 import torch
 
 own = False
@@ -151,8 +152,8 @@ def prepare(case, seed):
         at += c
     s = dict(case=case, table=table.to(DEV), max_seq=max_seq)
     s["before"] = torch.tensor(before, dtype=torch.int32, device=DEV)
-    s["after_host"] = [t + n for t, n in zip(before, new)]
-    s["after"] = torch.tensor(s["after_host"], dtype=torch.int32, device=DEV)
+    s["after_host"] = np.array([t + n for t, n in zip(before, new)], np.int32)
+    s["after"] = torch.from_numpy(s["after_host"]).to(DEV)
     s["new"] = torch.tensor(new, dtype=torch.int32, device=DEV) if case.get("pad") else None
     # keys of one page resemble each other, as a passage's keys do
     k = normal(n_pages, Hk, P, D).mul_(0.8).add_(normal(n_pages, Hk, 1, D), alpha=0.6)
@@ -186,7 +187,7 @@ def prepare(case, seed):
         s["store"] = mugen_amd.PagedStore(s["k"], s["v"], s["table"], max_seq, k_exp=s["k_exp"], v_exp=s["v_exp"],
                                           tail_k=s["tail_k"], tail_v=s["tail_v"], k_range=s["ranges"])
         if op in ("decode", "sparse"):
-            s["ws"] = s["store"].attention_workspace(B, L, H, n_select=case.get("chosen", 0))
+            s["ws"] = s["store"].attention_workspace(L, H, n_select=case.get("chosen", 0))
         elif op == "prefill":
             s["ws"] = s["store"].prefill_workspace(L, H, s["start"])
     return s
@@ -464,7 +465,7 @@ def exact(case, seed):
         return torch.stack([_attend(s["q"][i], k[:s["start"] + i + 1], v[:s["start"] + i + 1]) for i in range(L)])
     out = s["out"].double()
     for b in range(B):
-        T = s["after_host"][b]
+        T = int(s["after_host"][b])
         n = int(s["new"][b]) if s["new"] is not None else L
         if n == 0:
             continue
