@@ -712,7 +712,7 @@ static int gqa_prefill_validate(const mugen_attn_gqa_prefill_args* a) {
     if (!a->q || !a->k || !a->v || !a->out) return fail(MUGEN_ATTN_E_INVALID, "gqa_prefill: null tensor pointer");
     if (a->n_tokens < 0 || a->n_heads <= 0 || a->n_kv_heads <= 0 || a->kv_len < 0 || a->start_pos < 0)
         return fail(MUGEN_ATTN_E_INVALID, "gqa_prefill: negative size");
-    if (a->n_heads % a->n_kv_heads) return fail(MUGEN_ATTN_E_INVALID, "gqa_prefill: n_heads % n_kv_heads != 0");
+    if (a->n_heads % a->n_kv_heads) return fail(MUGEN_ATTN_E_INVALID, "gqa_prefill: n_heads %% n_kv_heads != 0");
     if (a->n_heads / a->n_kv_heads > 16)
         return fail(MUGEN_ATTN_E_UNSUPPORTED, "gqa_prefill: n_heads/n_kv_heads > 16");
     if (a->n_heads / a->n_kv_heads > 8 && a->kernel == MUGEN_ATTN_PREFILL_KERNEL_BLOCK)
