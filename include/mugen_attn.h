@@ -31,6 +31,8 @@
  *     (metal_compute.h:84-89); the C++ adapter mugen_attn.hpp maps codes +
  *     message back to that shape;
  *   - calls on distinct streams with distinct workspaces are thread-safe.
+ *
+ * The paged K/V cache is in mugen_attn_paged.h.
  */
 #ifndef MUGEN_ATTN_H
 #define MUGEN_ATTN_H

@@ -49,6 +49,18 @@ EXPORTS = (
     "mugen_attn_timing_reset",
 )
 
+# every symbol include/mugen_attn_paged.h declares
+EXPORTS_PAGED = (
+    "mugen_attn_kv_paged_append",
+    "mugen_attn_gqa_decode_paged_workspace_size",
+    "mugen_attn_gqa_decode_paged",
+    "mugen_attn_page_select_workspace_size",
+    "mugen_attn_page_select",
+    "mugen_attn_gqa_prefill_paged_workspace_size",
+    "mugen_attn_gqa_prefill_paged",
+)
+PAGED_MAX_Q = 64  # MUGEN_ATTN_PAGED_MAX_Q
+
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
@@ -143,6 +155,45 @@ class MlaProjectArgs(ctypes.Structure):
     ]
 
 
+class KvPages(ctypes.Structure):
+    _fields_ = [
+        ("k_pages", _vp), ("v_pages", _vp), ("k_exp", _vp), ("v_exp", _vp), ("tail_k", _vp), ("tail_v", _vp),
+        ("k_range", _vp), ("page_table", _vp), ("table_stride", _i64), ("tail_seq_stride", _i64),
+        ("n_seq", _i32), ("n_pages", _i32), ("page_tokens", _i32), ("page_bits", _i32), ("ring", _i32),
+        ("n_kv_heads", _i32), ("head_dim", _i32), ("max_seq_len", _i32), ("dtype", _i32),
+    ]
+
+
+class KvPagedAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("store", KvPages), ("k_new", _vp), ("v_new", _vp), ("q", _vp), ("q_out", _vp), ("seq_lens", _vp),
+        ("new_lens", _vp), ("seq_lens_out", _vp), ("k_stride", _i64), ("v_stride", _i64), ("q_stride", _i64),
+        ("n_new", _i32), ("n_heads", _i32), ("rope_dim", _i32), ("rope", RopeParams),
+    ]
+
+
+class GqaDecodePagedArgs(ctypes.Structure):
+    _fields_ = [
+        ("store", KvPages), ("q", _vp), ("out", _vp), ("seq_lens", _vp), ("q_lens", _vp), ("pages", _vp),
+        ("n_select", _i32), ("q_len", _i32), ("n_heads", _i32), ("num_splits", _i32), ("scale", _f32),
+        ("out_dtype", _i32), ("seq_lens_host", _vp),
+    ]
+
+
+class PageSelectArgs(ctypes.Structure):
+    _fields_ = [
+        ("store", KvPages), ("q", _vp), ("pages", _vp), ("seq_lens", _vp), ("q_lens", _vp), ("q_len", _i32),
+        ("n_heads", _i32), ("n_select", _i32), ("n_first", _i32), ("n_last", _i32),
+    ]
+
+
+class GqaPrefillPagedArgs(ctypes.Structure):
+    _fields_ = [
+        ("store", KvPages), ("q", _vp), ("out", _vp), ("seq", _i32), ("n_tokens", _i32), ("start_pos", _i32),
+        ("n_heads", _i32), ("scale", _f32), ("out_dtype", _i32),
+    ]
+
+
 class MugenAttnError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"[{code}] {msg}")
@@ -205,6 +256,13 @@ def lib(path: str | None = None) -> ctypes.CDLL:
         L.mugen_attn_seq_advance.restype = ctypes.c_int
         L.mugen_attn_scatter_kv.argtypes = [_vp, _vp, ctypes.c_uint64, ctypes.c_uint64, _vp]
         L.mugen_attn_scatter_kv.restype = ctypes.c_int
+        L.mugen_attn_kv_paged_append.argtypes = [ctypes.POINTER(KvPagedAppendArgs), _vp]
+        L.mugen_attn_kv_paged_append.restype = ctypes.c_int
+        for name, args in (("gqa_decode_paged", GqaDecodePagedArgs), ("page_select", PageSelectArgs),
+                           ("gqa_prefill_paged", GqaPrefillPagedArgs)):
+            size, call = getattr(L, f"mugen_attn_{name}_workspace_size"), getattr(L, f"mugen_attn_{name}")
+            size.argtypes, size.restype = [ctypes.POINTER(args)], ctypes.c_size_t
+            call.argtypes, call.restype = [ctypes.POINTER(args), _vp, ctypes.c_size_t, _vp], ctypes.c_int
         L.mugen_attn_last_error.restype = ctypes.c_char_p
         L.mugen_attn_version.restype = ctypes.c_char_p
         L.mugen_attn_timing_enable.argtypes = [ctypes.c_int]

@@ -18,6 +18,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "capi_common.h"
 #include "common.h"
 #include "kernels.h"
 #include "prefill_rules.h"
@@ -28,7 +29,7 @@ namespace mugen_attn {
 
 static thread_local std::string g_last_error;
 
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
     char buf[512];
     va_list ap;
     va_start(ap, fmt);
@@ -38,7 +39,7 @@ static int fail(int code, const char* fmt, ...) {
     return code;
 }
 
-static int hip_status(hipError_t e, const char* what) {
+int hip_status(hipError_t e, const char* what) {
     if (e == hipSuccess) return MUGEN_ATTN_OK;
     return fail(MUGEN_ATTN_E_HIP, "%s: %s", what, hipGetErrorString(e));
 }

@@ -1,0 +1,280 @@
+// page_select.hip -- the choice of the pages a query reads
+// (mugen_attn_page_select): a score kernel over the page ranges, then a top-k per
+// (query, kv head).
+//
+// Score.  sum over heads and dims of max(q min, q max) = Q-.min + Q+.max with
+// Q-, Q+ the sums over the group's heads of the negative and the positive parts
+// of q: one product of 2 * head_dim terms per page whatever the group's size.
+// In 64 bits: 16-bit factors make 22-bit products, so the sums come out the same in
+// any order but for terms 2^30 apart, and a page next to the border does not change
+// sides with the kernel's tiling.  16 lanes take a page (2 * head_dim contiguous values), 4 pages
+// a wave instruction; every query of a sequence is scored from one read.
+// Bound: HBM (4 * head_dim bytes a page and kv head).
+//
+// Choice.  Scores become 64-bit integers of the same order, held in registers.  A
+// radix select finds the border: 8 bits a pass from the highest bit in which any two
+// candidates differ, ended as soon as a digit's bin is taken whole, so that a few
+// passes do for scores that are spread.  Equal keys at the border are taken from
+// the lowest page on; two ballots and one scan then place the ascending list.
+#include "paged.h"
+
+namespace mugen_attn {
+namespace {
+
+__device__ __forceinline__ double row_sum16(double v) {  // over the 16 lanes of a row, in every lane
+    auto step = [&](auto ctrl) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, decltype(ctrl)::value, 0xF, 0xF, false);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), decltype(ctrl)::value, 0xF, 0xF, false);
+        v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    };
+    step(std::integral_constant<int, 0x128>{});  // row rotations by 8, 4, 2, 1
+    step(std::integral_constant<int, 0x124>{});
+    step(std::integral_constant<int, 0x122>{});
+    step(std::integral_constant<int, 0x121>{});
+    return v;
+}
+
+// what query i of sequence b sees
+struct Seen {
+    int n;      // new tokens of the sequence
+    int pages;  // pages that query i sees
+};
+__device__ __forceinline__ int select_len(const PageSelectParams& p, int b) { return clamp_len(p.seq_lens[b], p.st.max_T); }
+__device__ __forceinline__ int select_new(const PageSelectParams& p, int b) {
+    return p.q_lens ? min(max(p.q_lens[b], 0), p.q_len) : p.q_len;
+}
+__device__ __forceinline__ int pages_seen(const PageSelectParams& p, int T, int n, int i) {
+    return (max(T - n + i + 1, 0) + (1 << p.st.p_shift) - 1) >> p.st.p_shift;
+}
+
+constexpr int kScorePages = 64;  // pages of a score workgroup: 16 a step
+constexpr int kScoreQueries = 8;  // queries whose Q-, Q+ are held at a time
+
+template <int D, int DT>
+__global__ __launch_bounds__(256) void page_score_kernel(PageSelectParams p) {
+    constexpr int C = 2 * D / 128;  // 16-byte loads of a lane per page
+    constexpr int STEPS = kScorePages / 16;
+    __shared__ double Q[kScoreQueries][2 * D];
+    const int kvh = blockIdx.y, b = blockIdx.z, page0 = blockIdx.x * kScorePages;
+    const int T = select_len(p, b), n = select_new(p, b);
+    if (n == 0) return;
+    // candidates of the last query, the one that sees most
+    const int end = pages_seen(p, T, n, n - 1) - p.n_last;
+    if (page0 >= end || page0 + kScorePages <= p.n_first || end + p.n_last <= p.n_select) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15;
+    // this wave's pages: page0 + 16 * step + 4 * wave + lane / 16
+    u32x4_t raw[STEPS][C];
+    bool there[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) {
+        const int page = page0 + 16 * s + 4 * wave + (lane >> 4);
+        int phys = -1;
+        if (page < end) phys = checked_page(p.st.table[b * p.st.table_stride + page], p.st.n_pages);
+        there[s] = phys >= 0;
+        const uint16_t* src = p.st.k_range + ((int64_t)max(phys, 0) * p.st.Hk + kvh) * 2 * D;
+#pragma unroll
+        for (int c = 0; c < C; c++) raw[s][c] = load16(src + 8 * (16 * c + l16));
+    }
+    for (int i0 = 0; i0 < n; i0 += kScoreQueries) {
+        const int ni = min(kScoreQueries, n - i0);
+        __syncthreads();
+        for (int x = threadIdx.x; x < ni * D; x += 256) {
+            const int i = x / D, d = x - i * D;
+            const uint16_t* q = p.q + (((int64_t)b * p.q_len + i0 + i) * p.H + (int64_t)kvh * p.G) * D + d;
+            double neg = 0.0, pos = 0.0;
+            for (int h = 0; h < p.G; h++) {
+                const double v = (double)to_f32<DT>(q[h * D]);
+                if (v < 0.0) neg += v;
+                else pos += v;  // (a NaN too)
+            }
+            Q[i][d] = neg;
+            Q[i][D + d] = pos;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            double x[8 * C];
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[8 * c + 2 * e] = (double)lo_f32<DT>(raw[s][c][e]);
+                    x[8 * c + 2 * e + 1] = (double)hi_f32<DT>(raw[s][c][e]);
+                }
+            const int page = page0 + 16 * s + 4 * wave + (lane >> 4);
+            for (int i = 0; i < ni; i++) {
+                double sum = 0.0;
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) sum = fma(Q[i][8 * (16 * c + l16) + e], x[8 * c + e], sum);
+                sum = row_sum16(sum) + 0.0;  // (-0 counts as 0)
+                uint64_t key = __builtin_bit_cast(uint64_t, sum);
+                key = sum != sum ? ~0ull : (key >> 63) ? ~key : key | (1ull << 63);
+                if (!there[s]) key = 0;
+                if (l16 == 0 && page < end)
+                    p.keys[(((int64_t)b * p.q_len + i0 + i) * p.st.Hk + kvh) * p.max_pages + page] = key;
+            }
+        }
+    }
+}
+
+template <int WAVES, int KPT>
+__global__ __launch_bounds__(64 * WAVES) void page_select_kernel(PageSelectParams p) {
+    constexpr int NT = 64 * WAVES;
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t counts[KPT * WAVES];
+    __shared__ uint64_t red[2 * WAVES];
+    __shared__ int pick[2];
+    const int kvh = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int T = select_len(p, b), n = select_new(p, b);
+    if (i >= n) return;
+    int32_t* out = p.pages + (((int64_t)b * p.q_len + i) * p.st.Hk + kvh) * p.n_select;
+    const int pages = pages_seen(p, T, n, i);
+    if (pages <= p.n_select) {  // all of them
+        for (int x = tid; x < p.n_select; x += NT) out[x] = x < pages ? x : -1;
+        return;
+    }
+    const int first = p.n_first, end = pages - p.n_last;  // candidates [first, end)
+    int need = p.n_select - p.n_first - p.n_last;
+    const uint64_t* keys = p.keys + (((int64_t)b * p.q_len + i) * p.st.Hk + kvh) * p.max_pages;
+    uint64_t key[KPT];
+    uint64_t all = ~0ull, any = 0;  // bits set in every / in some candidate
+#pragma unroll
+    for (int m = 0; m < KPT; m++) {
+        const int x = m * NT + tid;
+        key[m] = 0;
+        if (x >= first && x < end) {
+            key[m] = keys[x];
+            all &= key[m];
+            any |= key[m];
+        }
+    }
+    for (int d = 32; d; d >>= 1) {
+        all &= __shfl_xor(all, d, 64);
+        any |= __shfl_xor(any, d, 64);
+    }
+    if (lane == 0) {
+        red[2 * w] = all;
+        red[2 * w + 1] = any;
+    }
+    __syncthreads();
+    all = ~0ull, any = 0;
+#pragma unroll
+    for (int x = 0; x < WAVES; x++) {
+        all &= red[2 * x];
+        any |= red[2 * x + 1];
+    }
+    // key >> shift > border: taken; == border: `need` of them
+    const uint64_t differ = all ^ any;
+    int shift = differ ? 64 - __builtin_clzll(differ) : 0;
+    uint64_t border = shift < 64 ? any >> shift : 0;  // the bits that all share
+    bool whole = need == 0 || need == end - first;    // the bin is taken whole, or not at all
+    if (need == 0) {                                  // (first and last fill the list)
+        shift = 0;
+        border = ~0ull;
+        whole = false;
+    }
+    while (!whole && shift > 0 && need > 0) {
+        const int bits = min(8, shift), next = shift - bits;
+        for (int x = tid; x < 256; x += NT) hist[x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < KPT; m++) {
+            const int x = m * NT + tid;
+            if (x >= first && x < end && (shift == 64 || key[m] >> shift == border))
+                atomicAdd(&hist[(key[m] >> next) & ((1u << bits) - 1)], 1u);
+        }
+        __syncthreads();
+        if (w == 0) {  // the bin, from the top, that holds the need-th: lane l has bins 255 - 4l .. 252 - 4l
+            uint32_t c[4], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                c[e] = hist[255 - 4 * lane - e];
+                sum += c[e];
+            }
+            const int incl = wave_scan_i32((int)sum);
+            const uint64_t past = __ballot(incl >= need);
+            if (lane == __builtin_ctzll(past)) {
+                int above = incl - (int)sum, e = 0;
+                while (e < 3 && above + (int)c[e] < need) above += (int)c[e++];
+                pick[0] = 255 - 4 * lane - e;
+                pick[1] = need - above;
+                hist[255 - 4 * lane - e] = c[e] == (uint32_t)(need - above) ? 0xffffffffu : c[e];
+            }
+        }
+        __syncthreads();
+        const int bin = pick[0];
+        need = pick[1];
+        whole = hist[bin] == 0xffffffffu;
+        border = (shift == 64 ? 0 : border << bits) | (uint64_t)bin;
+        shift = next;
+        __syncthreads();
+    }
+    // places: a ballot per 64 pages, their counts scanned in page order
+    auto place = [&](auto taken, uint32_t (&before)[KPT]) {
+        uint64_t bal[KPT];
+#pragma unroll
+        for (int m = 0; m < KPT; m++) {
+            bal[m] = __ballot(taken(m));
+            if (lane == 0) counts[m * WAVES + w] = (uint32_t)__popcll(bal[m]);
+        }
+        __syncthreads();
+        if (w == 0) {
+            int carry = 0;
+            for (int x0 = 0; x0 < KPT * WAVES; x0 += 64) {
+                const int c = x0 + lane < KPT * WAVES ? (int)counts[x0 + lane] : 0;
+                const int incl = wave_scan_i32(c);
+                if (x0 + lane < KPT * WAVES) counts[x0 + lane] = (uint32_t)(carry + incl - c);
+                carry += __builtin_amdgcn_readlane(incl, 63);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < KPT; m++)
+            before[m] = counts[m * WAVES + w] + (uint32_t)__popcll(bal[m] & ((1ull << lane) - 1));
+        __syncthreads();
+    };
+    uint32_t before[KPT];
+    auto cand = [&](int m) { return m * NT + tid >= first && m * NT + tid < end; };
+    auto at_border = [&](int m) { return cand(m) && (shift == 64 || key[m] >> shift == border); };
+    if (!whole) place(at_border, before);  // equal keys: the lowest pages
+    bool tie[KPT];
+#pragma unroll
+    for (int m = 0; m < KPT; m++) tie[m] = at_border(m) && (whole || before[m] < (uint32_t)need);
+    auto taken = [&](int m) {
+        const int x = m * NT + tid;
+        if (x < first || (x >= end && x < pages)) return true;
+        return cand(m) && (tie[m] || (shift < 64 && key[m] >> shift > border));
+    };
+    place(taken, before);
+#pragma unroll
+    for (int m = 0; m < KPT; m++)
+        if (taken(m) && before[m] < (uint32_t)p.n_select) out[before[m]] = m * NT + tid;
+}
+
+template <int D>
+hipError_t launch_score_d(const PageSelectParams& p, int dt, hipStream_t st, KernelTimer* t) {
+    const dim3 grid((p.max_pages + kScorePages - 1) / kScorePages, p.st.Hk, p.B);
+    if (dt == DT_F16) return launch_k(t, "page_score", page_score_kernel<D, DT_F16>, grid, dim3(256), st, p);
+    return launch_k(t, "page_score", page_score_kernel<D, DT_BF16>, grid, dim3(256), st, p);
+}
+
+}  // namespace
+
+hipError_t launch_page_score(const PageSelectParams& p, int D, int dt, hipStream_t st, KernelTimer* t) {
+    if (D == 256) return launch_score_d<256>(p, dt, st, t);
+    if (D == 128) return launch_score_d<128>(p, dt, st, t);
+    return launch_score_d<64>(p, dt, st, t);
+}
+
+hipError_t launch_page_select(const PageSelectParams& p, hipStream_t st, KernelTimer* t) {
+    const dim3 grid(p.st.Hk, p.q_len, p.B);
+    if (p.max_pages <= 1024) return launch_k(t, "page_select", page_select_kernel<4, 4>, grid, dim3(256), st, p);
+    if (p.max_pages <= 4096) return launch_k(t, "page_select", page_select_kernel<16, 4>, grid, dim3(1024), st, p);
+    return launch_k(t, "page_select", page_select_kernel<16, 16>, grid, dim3(1024), st, p);
+}
+
+}  // namespace mugen_attn

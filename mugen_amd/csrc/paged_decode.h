@@ -1,0 +1,598 @@
+// paged_decode.h -- split-K GQA attention over the paged K/V cache, the kernel
+// behind paged_decode16.hip (16-bit pages) and paged_decode8.hip (E4M3 pages).
+//
+// Semantics: softmax(q.K^T * scale) V with fp32 accumulation, kv head = h /
+// (H / Hk), for 1..n new tokens per sequence, causal among them, over the pages
+// of the sequence or over a page list per query (LIST).
+//
+// Design (HBM-bound: each K and V byte is read once):
+//  * one workgroup = (context split, kv head, sequence, row block); its rows
+//    are (token, head of the group) pairs, up to NR * 16 of them served from
+//    one read of K and V (a verify step's tokens share it);
+//  * 4 waves; wave w takes the 32-token tiles w, w+4, ... of the split and
+//    loads the next tile while computing the current one.  A page holds whole
+//    tiles, so a tile's address is one page id away: the ids (and the 8-bit
+//    scales) of 64 pages sit in one register across the lanes, read with
+//    v_readlane, the next 64 loaded ahead;
+//  * S^T[32 tokens x 16 rows] = K.Q^T and O^T[D x 16 rows] += V^T.P^T on MFMA
+//    16x16x32.  K rows are the A operand straight from memory, in the token order
+//    that leaves each lane 8 consecutive tokens of its row (A row m of block nb
+//    is token 8*(m/4) + 4*nb + m%4) and in the dim order that makes a lane's
+//    8-bit loads 16 bytes wide (k-step 2j+h, lane group g: dims 64j + 16g + 8h
+//    .. +7); q is loaded in the same order;
+//  * 8-bit V pages are stored [dim][32 tokens], so V^T is an A operand straight
+//    from memory too: no LDS in the main loop.  Codes are expanded in registers
+//    (v_cvt_scalef32_pk), V's scale in that conversion, K's with the softmax scale;
+//  * 16-bit V rows (16-bit pages, and the ring behind the last whole 8-bit page)
+//    go through a per-wave LDS buffer and ds_read_b64_tr_b16;
+//  * online softmax in the exp2 domain with a lazy max (a row is re-based only
+//    when a weight would exceed 2^8); P is fp16, or bf16 hi + lo;
+//  * a V row that a query does not see is zeroed before its product, not only
+//    weighted 0: 0 * inf is NaN.  Tiles that reach past the first query's last token
+//    are checked for values that are not finite; where one is met, each token's
+//    rows get their own product with the later rows zeroed;
+//  * the 4 waves merge (m, l, o) through LDS; with one split the result is
+//    stored, otherwise fp32 partials go to the workspace and the combine merges
+//    them.
+#pragma once
+#include "paged.h"
+
+namespace mugen_attn {
+namespace paged {
+
+// 16-byte chunk c of staged V row r sits at chunk c ^ swz(r): the transpose
+// reads of lane groups g, g+1 (rows 8g + r', r' < 4, chunks 2d, 2d + 1) then
+// hit distinct banks (rows of 128 B at D = 64, 256 B or more above)
+template <int D>
+__device__ constexpr int swz(int r) {
+    if constexpr (D == 64) return (((r >> 1) & 1) * 2) ^ (((r >> 3) & 1) * 4) ^ ((r >> 4) & 1);
+    else return ((r & 1) * 2) ^ (((r >> 1) & 1) * 4) ^ (((r >> 3) & 1) * 8) ^ ((r >> 4) & 1);
+}
+
+// any 16-bit element (inf, NaN) / E4M3 code (NaN) of w that is not finite
+template <int DT>
+__device__ __forceinline__ bool bad16(uint32_t w) {
+    if constexpr (DT == DT_F16) return (((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0;
+    else return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0;
+}
+__device__ __forceinline__ bool bad8(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
+
+// tokens the new tokens' queries see: sequence length and count
+struct Lens {
+    int T, n;
+};
+__device__ __forceinline__ Lens seq_lens_of(const PagedDecodeParams& p, int b) {
+    Lens r;
+    r.T = p.seq_lens ? clamp_len(p.seq_lens[b], p.st.max_T) : p.fixed_T;
+    r.n = p.q_lens ? min(max(p.q_lens[b], 0), p.q_len) : p.q_len;
+    return r;
+}
+
+// list entries a query that sees `limit` tokens may use
+__device__ __forceinline__ int list_len(const PagedDecodeParams& p, int limit) {
+    return min(p.n_sel, (max(limit, 0) + (1 << p.st.p_shift) - 1) >> p.st.p_shift);
+}
+
+// tokens in sequence (LIST: query) j's key range
+template <bool LIST>
+__device__ __forceinline__ int range_of(const PagedDecodeParams& p, int j) {
+    if constexpr (LIST) {
+        const int b = j / p.q_len, i = j - b * p.q_len;
+        const Lens s = seq_lens_of(p, b);
+        return i < s.n ? list_len(p, s.T - s.n + i + 1) << p.st.p_shift : 0;
+    } else {
+        const Lens s = seq_lens_of(p, j);
+        return s.n > 0 ? s.T : 0;
+    }
+}
+
+template <bool LIST>
+__device__ __forceinline__ int plan(const PagedDecodeParams& p) {
+    auto units = [&](int j) { return (range_of<LIST>(p, j) + 31) >> 5; };
+    return plan_chunk_device<1>(
+        p.B, p.st.Hk * p.nrb, p.budget, [](int) { return 2; }, p.num_splits, units,
+        [&](int j, int c, float rc) { return max(1, ceil_div_f(units(j), c, rc)); });
+}
+
+// two waves per SIMD where a wave's operands fit in half the registers
+template <int D, int DT, bool BITS8, int NR, bool LIST>
+constexpr int waves_per_eu() {
+    return D > 128 || NR > (BITS8 ? 2 : 1) ? 1 : 2;
+}
+
+template <int D, int DT, bool BITS8, int NR, bool LIST>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves_per_eu<D, DT, BITS8, NR, LIST>()))) void
+paged_decode_kernel(PagedDecodeParams p) {
+    constexpr int KK = D / 32;          // MFMA k-steps of S
+    constexpr int KJ = D / 64;          // 16-byte loads of an 8-bit K row per lane
+    constexpr int DB = D / 16;          // 16-dim blocks of O^T
+    constexpr int RB = 2 * D;           // bytes of a staged V row
+    constexpr int VL = 32 * RB / 1024;  // 16-byte V loads per lane per 16-bit tile
+    constexpr int RPL = 1024 / RB;      // V rows per load instruction
+    constexpr int NP = p_terms<DT>();
+    constexpr float kHeadroom = 8.f;
+    constexpr int kNever = 0x3fffffff;  // a tile that no row sees
+    constexpr int STAGE = 4 * 32 * RB;
+    constexpr int OROW = D + 4;
+    constexpr int MERGE = 4 * 16 * OROW * 4 + 3 * 4 * 16 * 4 + 2 * 16 * 4;
+    __shared__ __attribute__((aligned(16))) char lds[STAGE > MERGE ? STAGE : MERGE];
+
+    const int Hk = p.st.Hk, ps = p.st.p_shift, P = 1 << ps;
+    const int chunk = p.chunk ? p.chunk : plan<LIST>(p);
+    int j = -1, r = 0;
+    const int mult = Hk * p.nrb;
+    auto items = [&](int x) {
+        const int len = range_of<LIST>(p, x);
+        return (len > 0 ? (len + chunk - 1) / chunk : 1) * mult;
+    };
+    if (!find_sequence(p.B, (int)blockIdx.x, items, j, r)) return;  // grid padding
+    const int s = r / mult, kr = r - s * mult, kvh = kr / p.nrb, rb = kr - kvh * p.nrb;
+    if (p.num_splits > 1 && s >= p.num_splits) return;  // past the workspace's stride
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int b = LIST ? j / p.q_len : j, i0 = LIST ? j - b * p.q_len : 0;
+    const Lens len = seq_lens_of(p, b);
+    const int T = len.T;
+    const int range = range_of<LIST>(p, j);
+    const int t_begin = s * chunk, t_end = min(t_begin + chunk, range);
+    if (p.chunk == 0 && blockIdx.x == 0 && threadIdx.x == 0) *p.plan = chunk;  // for the merge
+    if (p.num_splits > 1 && t_begin >= t_end) return;  // nothing to see: the merge skips it
+    const int G = p.G, first_row = rb * NR * 16, n_rows = (LIST ? 1 : len.n) * G;
+    if (first_row >= n_rows) return;  // rows of tokens that are not there
+
+    // the lane's rows 16 * rr + n: their queries, and how many tokens they see
+    u32x4_t qf[NR][KK];
+    int limit[NR], tok[NR];
+    int low = T;  // the first query's tokens: tiles below it are seen by every row
+#pragma unroll
+    for (int rr = 0; rr < NR; rr++) {
+        const int row = first_row + 16 * rr + n;
+        const int i = LIST ? i0 : row / G, h = LIST ? row : row - i * G;
+        const bool live = row < n_rows;
+        tok[rr] = live ? i : -1;
+        limit[rr] = live ? max(T - len.n + i + 1, 0) : 0;
+        const uint16_t* qp = p.q + (((int64_t)b * p.q_len + i) * p.H + kvh * G + h) * D;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++)
+            qf[rr][kk] = live ? load16(qp + 64 * (kk >> 1) + 16 * g + 8 * (kk & 1)) : u32x4_t{0, 0, 0, 0};
+    }
+    const int tok_first = LIST ? i0 : first_row / G;
+    const int tok_last = LIST ? i0 : (min(first_row + NR * 16, n_rows) - 1) / G;
+    low = max(T - len.n + tok_first + 1, 0);
+
+    f32x4_t o[NR][DB];  // lane (g, n): O[row 16 rr + n][16d + 4g + i]
+    float m_run[NR], l_part[NR];
+#pragma unroll
+    for (int rr = 0; rr < NR; rr++) {
+        m_run[rr] = kNegInf;
+        l_part[rr] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; d++) o[rr][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // ---- page ids: lane l holds page first_page + l of the split, physical
+    // (-1: not there), logical (LIST), and the two exponents
+    const int first_page = t_begin >> ps, end_page = (t_end + P - 1) >> ps;
+    const int32_t* table = p.st.table + b * p.st.table_stride;
+    const int whole = T >> ps;  // 8-bit: pages before it are whole, page `whole` is in the ring
+    const int my_limit = LIST ? max(T - len.n + i0 + 1, 0) : T;
+    const int32_t* list = LIST ? p.sel + (((int64_t)b * p.q_len + i0) * Hk + kvh) * p.n_sel : nullptr;
+    struct Ids {
+        int phys, lp;
+        uint32_t exps;
+    };
+    auto load_ids = [&](int page0) {
+        Ids x{-1, -1, 0};
+        const int k = page0 + lane;
+        if (k < end_page) {
+            int lp = k;
+            if constexpr (LIST) {
+                lp = list[k];
+                const int before = k > 0 ? list[k - 1] : -1;
+                if (lp <= before || lp >= (my_limit + P - 1) >> ps) lp = -1;
+            }
+            if (lp >= 0) {
+                if (!BITS8 || lp < whole) x.phys = checked_page(table[lp], p.st.n_pages);
+                x.lp = lp;
+            }
+        }
+        if constexpr (BITS8) {
+            if (x.phys >= 0) {
+                const int64_t e = (int64_t)x.phys * Hk + kvh;
+                x.exps = (uint32_t)p.st.k_exp[e] | ((uint32_t)p.st.v_exp[e] << 8);
+            }
+        }
+        return x;
+    };
+    Ids ids = load_ids(first_page), ids_next{-1, -1, 0};
+    int ids_at = first_page;
+    if (ids_at + 64 < end_page) ids_next = load_ids(ids_at + 64);
+
+    // a tile's place: its page, where it starts in it, its first token
+    struct Tile {
+        int phys, off, t0;
+        uint32_t exps;
+    };
+    auto find_tile = [&](int t) {  // t: wave-uniform, ascending over the calls
+        const int k = t >> ps;
+        while (k >= ids_at + 64) {
+            ids = ids_next;
+            ids_at += 64;
+            if (ids_at + 64 < end_page) ids_next = load_ids(ids_at + 64);
+        }
+        Tile x;
+        x.phys = __builtin_amdgcn_readlane(ids.phys, k - ids_at);
+        x.off = t & (P - 1);
+        const int lp = LIST ? __builtin_amdgcn_readlane(ids.lp, k - ids_at) : k;
+        x.t0 = x.phys >= 0 ? (lp << ps) + x.off : kNever;
+        x.exps = BITS8 ? (uint32_t)__builtin_amdgcn_readlane((int)ids.exps, k - ids_at) : 0u;
+        return x;
+    };
+
+    // ---- softmax of one tile's scores (lane: 8 consecutive tokens of its
+    // rows), P as the B operand
+    auto softmax_tile = [&](f32x4_t (&sacc)[NR][2], int t0, float scale, u32x4_t (&pf)[NR][NP]) {
+#pragma unroll
+        for (int rr = 0; rr < NR; rr++) {
+            float x[8];
+            float smax = kNegInf;
+            const int seen = limit[rr] - t0 - 8 * g;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = e < seen ? sacc[rr][e >> 2][e & 3] * scale : kNegInf;
+                x[e] = v;
+                smax = fmaxf(smax, v);
+            }
+            if (__any(smax > m_run[rr] + kHeadroom)) {  // re-base the rows (wave-uniform branch)
+                const float m_new = fmaxf(m_run[rr], max_x32(max_x16(smax)));
+                if (m_new > m_run[rr]) {
+                    const float alpha = fast_exp2(m_run[rr] - m_new);  // 0 while m_run = -inf
+                    l_part[rr] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < DB; d++) o[rr][d] *= alpha;
+                    m_run[rr] = m_new;
+                }
+            }
+            const float nm = m_run[rr] == kNegInf ? 0.f : -m_run[rr];
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x[e] = fast_exp2(x[e] + nm);
+                sum += x[e];
+            }
+            l_part[rr] += sum;
+            split_p<DT, NP>(x, pf[rr]);
+        }
+    };
+    // O^T += V^T.P^T, V^T blocks from vt(d)
+    auto product = [&](auto vt, u32x4_t (&pf)[NR][NP]) {
+#pragma unroll
+        for (int d = 0; d < DB; d++) {
+            const u32x4_t a = vt(d);
+#pragma unroll
+            for (int rr = 0; rr < NR; rr++)
+#pragma unroll
+                for (int t = 0; t < NP; t++) o[rr][d] = mfma16x16x32<DT>(a, pf[rr][t], o[rr][d]);
+        }
+    };
+    // the same for the rows of token i alone (a lane holds one row of O; the
+    // others' weights are no zeros that would keep a NaN out)
+    auto product_of = [&](int i, auto vt, u32x4_t (&pf)[NR][NP]) {
+#pragma unroll
+        for (int d = 0; d < DB; d++) {
+            const u32x4_t a = vt(d);
+#pragma unroll
+            for (int rr = 0; rr < NR; rr++) {
+                f32x4_t x = o[rr][d];
+#pragma unroll
+                for (int t = 0; t < NP; t++) x = mfma16x16x32<DT>(a, pf[rr][t], x);
+                if (tok[rr] == i) o[rr][d] = x;
+            }
+        }
+    };
+
+    // ---- a tile of 16-bit rows: K [32][D] and V [32][D], rows `stride` apart
+    const int kr0 = 8 * (n >> 2) + (n & 3);  // + 4nb
+    auto load16_tile = [&](const uint16_t* kb, const uint16_t* vb, int stride, int last, u32x4_t (&kq)[2][KK],
+                           u32x4_t (&vq)[VL]) {
+#pragma unroll
+        for (int nb = 0; nb < 2; nb++) {
+            const int row = min(kr0 + 4 * nb, last) * stride;
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) kq[nb][kk] = load16(kb + row + 64 * (kk >> 1) + 16 * g + 8 * (kk & 1));
+        }
+#pragma unroll
+        for (int x = 0; x < VL; x++)
+            vq[x] = load16(vb + min(x * RPL + lane / (RB / 16), last) * stride + 8 * (lane % (RB / 16)));
+    };
+    char* stage = &lds[w * 32 * RB];
+    uint32_t st_off[VL], t_off[DB];
+#pragma unroll
+    for (int x = 0; x < VL; x++) {
+        const int row = x * RPL + lane / (RB / 16), c = lane % (RB / 16);
+        st_off[x] = row * RB + ((c ^ swz<D>(row)) * 16);
+    }
+    const int tr = 8 * g + (n >> 2);
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+        t_off[d] = tr * RB + (((2 * d + ((n & 3) >> 1)) ^ swz<D>(tr)) * 16) + 8 * (n & 1);
+    auto wave_sync = [] {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    auto staged = [&](int d) {
+        const u32x2_t lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(stage + t_off[d]));
+        const u32x2_t hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(stage + t_off[d] + 4 * RB));
+        return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+    };
+    // V rows from `seen` on zeroed
+    auto stage_rows = [&](u32x4_t (&vq)[VL], int seen) {
+#pragma unroll
+        for (int x = 0; x < VL; x++) {
+            const bool in = x * RPL + lane / (RB / 16) < seen;
+            *reinterpret_cast<u32x4_t*>(stage + st_off[x]) = in ? vq[x] : u32x4_t{0, 0, 0, 0};
+        }
+    };
+    auto compute16 = [&](u32x4_t (&kq)[2][KK], u32x4_t (&vq)[VL], int t0) {
+        const bool edge = t0 + 32 > low;
+        if (!edge) {
+#pragma unroll
+            for (int x = 0; x < VL; x++) *reinterpret_cast<u32x4_t*>(stage + st_off[x]) = vq[x];
+        }
+        f32x4_t sacc[NR][2];
+#pragma unroll
+        for (int rr = 0; rr < NR; rr++)
+#pragma unroll
+            for (int nb = 0; nb < 2; nb++) {
+                f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++) acc = mfma16x16x32<DT>(kq[nb][kk], qf[rr][kk], acc);
+                sacc[rr][nb] = acc;
+            }
+        u32x4_t pf[NR][NP];
+        softmax_tile(sacc, t0, p.scale_log2, pf);
+        if (edge) {
+            bool bad = false;
+#pragma unroll
+            for (int x = 0; x < VL; x++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) bad |= bad16<DT>(vq[x][e]);
+            if (tok_first != tok_last && __any(bad)) {
+                for (int i = tok_first; i <= tok_last; i++) {
+                    stage_rows(vq, T - len.n + i + 1 - t0);
+                    wave_sync();
+                    product_of(i, staged, pf);
+                    wave_sync();
+                }
+                return;
+            }
+            stage_rows(vq, (LIST ? my_limit : T - len.n + tok_last + 1) - t0);
+        }
+        wave_sync();
+        product(staged, pf);
+        wave_sync();
+    };
+
+    if constexpr (!BITS8) {
+        u32x4_t kf[2][KK], kn[2][KK], vf[VL], vn[VL];
+        auto load = [&](int t, u32x4_t (&kq)[2][KK], u32x4_t (&vq)[VL]) {
+            const Tile x = find_tile(t);
+            const int64_t at = ((((int64_t)max(x.phys, 0) * Hk + kvh) << ps) + x.off) * D;
+            // tokens past the sequence are not read: the last one instead
+            load16_tile(reinterpret_cast<const uint16_t*>(p.st.k) + at, reinterpret_cast<const uint16_t*>(p.st.v) + at, D,
+                        min(31, max(T - 1 - x.t0, 0)), kq, vq);
+            return x.t0;
+        };
+        int t = t_begin + 32 * w;
+        int t0 = kNever, t0_next = kNever;
+        if (t < t_end) t0 = load(t, kf, vf);
+        for (; t < t_end; t += 128) {
+            const bool more = t + 128 < t_end;
+            if (more) t0_next = load(t + 128, kn, vn);
+            compute16(kf, vf, t0);
+            if (more) {
+                t0 = t0_next;
+#pragma unroll
+                for (int nb = 0; nb < 2; nb++)
+#pragma unroll
+                    for (int kk = 0; kk < KK; kk++) kf[nb][kk] = kn[nb][kk];
+#pragma unroll
+                for (int x = 0; x < VL; x++) vf[x] = vn[x];
+            }
+        }
+    } else {
+        struct Raw {
+            u32x4_t k[2][KJ];
+            u32x2_t v[DB];
+        };
+        auto load = [&](int t, Raw& x) {
+            const Tile at = find_tile(t);
+            const int64_t base = ((((int64_t)max(at.phys, 0) * Hk + kvh) << ps) + at.off) * D;
+            const uint8_t* kb = p.st.k + base;
+            const uint8_t* vb = p.st.v + base;
+#pragma unroll
+            for (int nb = 0; nb < 2; nb++)
+#pragma unroll
+                for (int c = 0; c < KJ; c++) x.k[nb][c] = load16(kb + (kr0 + 4 * nb) * D + 64 * c + 16 * g);
+#pragma unroll
+            for (int d = 0; d < DB; d++) x.v[d] = load8(vb + (16 * d + n) * 32 + 8 * g);
+            return at;
+        };
+        // V codes of tokens from `seen` on zeroed (the lane's tokens 8g .. 8g+7)
+        auto keep = [&](u32x2_t v, int seen) {
+            const int k = min(max(seen - 8 * g, 0), 8);
+            const uint64_t mask = k >= 8 ? ~0ull : (1ull << (8 * k)) - 1;
+            return u32x2_t{v[0] & (uint32_t)mask, v[1] & (uint32_t)(mask >> 32)};
+        };
+        auto compute8 = [&](Raw& x, const Tile& at) {
+            const float ks = exp_scale(at.exps & 0xffu) * p.scale_log2, vs = exp_scale((at.exps >> 8) & 0xffu);
+            f32x4_t sacc[NR][2];
+#pragma unroll
+            for (int nb = 0; nb < 2; nb++) {
+                u32x4_t kf[KK];
+#pragma unroll
+                for (int c = 0; c < KJ; c++) {
+                    kf[2 * c] = cvt8_fp8<DT>(x.k[nb][c][0], x.k[nb][c][1], 1.0f);
+                    kf[2 * c + 1] = cvt8_fp8<DT>(x.k[nb][c][2], x.k[nb][c][3], 1.0f);
+                }
+#pragma unroll
+                for (int rr = 0; rr < NR; rr++) {
+                    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int kk = 0; kk < KK; kk++) acc = mfma16x16x32<DT>(kf[kk], qf[rr][kk], acc);
+                    sacc[rr][nb] = acc;
+                }
+            }
+            u32x4_t pf[NR][NP];
+            softmax_tile(sacc, at.t0, ks, pf);
+            if (at.t0 + 32 > low) {
+                bool bad = false;
+#pragma unroll
+                for (int d = 0; d < DB; d++) bad |= bad8(x.v[d][0]) | bad8(x.v[d][1]);
+                if (__any(bad)) {  // (a page that is not there: nothing seen, all zero)
+                    for (int i = tok_first; i <= tok_last; i++) {
+                        const int seen = T - len.n + i + 1 - at.t0;
+                        product_of(i, [&](int d) {
+                            const u32x2_t v = keep(x.v[d], seen);
+                            return cvt8_fp8<DT>(v[0], v[1], vs);
+                        }, pf);
+                    }
+                    return;
+                }
+            }
+            product([&](int d) { return cvt8_fp8<DT>(x.v[d][0], x.v[d][1], vs); }, pf);
+        };
+        // tiles in whole pages; the ring's page (dense: from token whole * P on;
+        // LIST: the last valid entry, met as a page that is not there) after them
+        const int end8 = LIST ? t_end : min(t_end, whole << ps);
+        int t = t_begin + 32 * w;
+        Raw cur, nxt;
+        Tile at{-1, 0, kNever, 0}, at_next{-1, 0, kNever, 0};
+        if (t < end8) at = load(t, cur);
+        for (; t < end8; t += 128) {
+            const bool more = t + 128 < end8;
+            if (more) at_next = load(t + 128, nxt);
+            compute8(cur, at);
+            if (more) {
+                cur = nxt;
+                at = at_next;
+            }
+        }
+        // ---- the open page
+        int open = LIST ? -1 : whole;  // its place in the range, in pages
+        if constexpr (LIST) {
+            // the lists ascend, so the open page can only be the last entry that counts
+            for (int k = first_page + lane; k < end_page; k += 64) {
+                const int lp = list[k], before = k > 0 ? list[k - 1] : -1;
+                if (lp == whole && lp > before && lp < (my_limit + P - 1) >> ps) open = k;
+            }
+            open = -wave_min_i32(-open);
+        }
+        open = __builtin_amdgcn_readfirstlane(open);
+        if (open >= first_page && open < end_page) {
+            // this wave's tiles of the page inside the split
+            const int lo = max(open << ps, t_begin), hi = min((open + 1) << ps, t_end);
+            int tt = t_begin + 32 * w;
+            if (tt < lo) tt += (lo - tt + 127) / 128 * 128;
+            for (; tt < hi; tt += 128) {
+                const int t0 = (whole << ps) + (tt & (P - 1));  // its first token
+                if (t0 >= T) break;
+                const int64_t ring_at = b * p.st.tail_stride + ((int64_t)(t0 & (p.st.ring - 1)) * Hk + kvh) * D;
+                u32x4_t kq[2][KK], vq[VL];
+                load16_tile(p.st.tail_k + ring_at, p.st.tail_v + ring_at, Hk * D, min(31, T - 1 - t0), kq, vq);
+                compute16(kq, vq, t0);
+            }
+        }
+    }
+
+    // ---- merge the 4 waves' (m, l, O) per row through LDS, a row block at a time
+    float* o_lds = reinterpret_cast<float*>(&lds[0]);  // [4][16][OROW]
+    float* m_lds = o_lds + 4 * 16 * OROW;              // [4][16]
+    float* l_lds = m_lds + 4 * 16;
+    float* f_lds = l_lds + 4 * 16;                     // [4][16]: the waves' factors
+    float* ml_out = f_lds + 4 * 16;                    // [16][2]: the row's (M, L)
+#pragma unroll
+    for (int rr = 0; rr < NR; rr++) {
+        if (first_row + 16 * rr >= n_rows) break;  // (uniform)
+        const float l = sum_x32(sum_x16(l_part[rr]));
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+            *reinterpret_cast<f32x4_t*>(&o_lds[(w * 16 + n) * OROW + 16 * d + 4 * g]) = o[rr][d];
+        if (g == 0) {
+            // (a NaN sum behind a maximum that no number set still counts)
+            m_lds[w * 16 + n] = l != l && m_run[rr] == kNegInf ? 0.f : m_run[rr];
+            l_lds[w * 16 + n] = l;
+        }
+        __syncthreads();
+        if (threadIdx.x < 16) {
+            const int h = threadIdx.x;
+            float M = kNegInf;
+#pragma unroll
+            for (int x = 0; x < 4; x++) M = fmaxf(M, m_lds[x * 16 + h]);
+            float f[4], L = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const float mw = m_lds[x * 16 + h];
+                f[x] = mw == kNegInf ? 0.f : fast_exp2(mw - M);
+                L += f[x] * l_lds[x * 16 + h];
+            }
+            const float c = p.num_splits == 1 ? (L > 0.f ? 1.f / L : L == L ? 0.f : L) : 1.f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) f_lds[x * 16 + h] = f[x] * c;
+            ml_out[2 * h] = M;
+            ml_out[2 * h + 1] = L;
+        }
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < 16 * D; idx += 256) {
+            const int h = idx / D, d = idx - h * D, row = first_row + 16 * rr + h;
+            if (row >= n_rows) break;
+            const int i = LIST ? i0 : row / G, hh = LIST ? row : row - i * G;
+            float O = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const float f = f_lds[x * 16 + h];
+                O += f == 0.f ? 0.f : f * o_lds[(x * 16 + h) * OROW + d];
+            }
+            const int64_t orow = ((int64_t)b * p.q_len + i) * p.H + kvh * G + hh;
+            if (p.num_splits == 1) {
+                if (p.out_dt == DT_F32) store_out<DT_F32>(p.out, orow * D + d, O);
+                else if (p.out_dt == DT_F16) store_out<DT_F16>(p.out, orow * D + d, O);
+                else store_out<DT_BF16>(p.out, orow * D + d, O);
+            } else {
+                const int64_t slot = orow * p.num_splits + s;
+                p.ws_o[slot * D + d] = O;
+                if (d == 0) {
+                    p.ws_ml[slot * 2] = ml_out[2 * h];
+                    p.ws_ml[slot * 2 + 1] = ml_out[2 * h + 1];
+                }
+            }
+        }
+    }
+}
+
+template <int D, int DT, bool BITS8>
+hipError_t launch_rows(const PagedDecodeParams& p, int nwg, int nr, hipStream_t st, KernelTimer* t) {
+    const dim3 grid(nwg), block(256);
+    if (p.sel) return launch_k(t, "gqa_decode_paged", paged_decode_kernel<D, DT, BITS8, 1, true>, grid, block, st, p);
+    if (nr == 1) return launch_k(t, "gqa_decode_paged", paged_decode_kernel<D, DT, BITS8, 1, false>, grid, block, st, p);
+    if constexpr (D <= 128)
+        if (nr == 4) return launch_k(t, "gqa_decode_paged", paged_decode_kernel<D, DT, BITS8, 4, false>, grid, block, st, p);
+    return launch_k(t, "gqa_decode_paged", paged_decode_kernel<D, DT, BITS8, 2, false>, grid, block, st, p);
+}
+
+template <bool BITS8>
+hipError_t launch_decode(const PagedDecodeParams& p, int nwg, int D, int dt, int nr, hipStream_t st, KernelTimer* t) {
+    auto by_dt = [&](auto d) {
+        constexpr int DD = decltype(d)::value;
+        return dt == DT_F16 ? launch_rows<DD, DT_F16, BITS8>(p, nwg, nr, st, t)
+                            : launch_rows<DD, DT_BF16, BITS8>(p, nwg, nr, st, t);
+    };
+    if (D == 256) return by_dt(std::integral_constant<int, 256>{});
+    if (D == 128) return by_dt(std::integral_constant<int, 128>{});
+    return by_dt(std::integral_constant<int, 64>{});
+}
+
+}  // namespace paged
+}  // namespace mugen_attn
