@@ -96,10 +96,10 @@ struct PagedGatherParams {
 
 hipError_t launch_paged_append(const PagedAppendParams& p, int D, int dt, bool bits8, hipStream_t st, KernelTimer* t);
 hipError_t launch_paged_gather(const PagedGatherParams& p, int D, int dt, bool bits8, hipStream_t st, KernelTimer* t);
-// nr: 16-row blocks of one workgroup (1, 2 or 4)
-hipError_t launch_paged_decode16(const PagedDecodeParams& p, int nwg, int D, int dt, int nr, hipStream_t st,
+// wr: 16-row blocks of one workgroup (1 .. 4; 1, 2 or 4 at head_dim 256)
+hipError_t launch_paged_decode16(const PagedDecodeParams& p, int nwg, int D, int dt, int wr, hipStream_t st,
                                  KernelTimer* t);
-hipError_t launch_paged_decode8(const PagedDecodeParams& p, int nwg, int D, int dt, int nr, hipStream_t st,
+hipError_t launch_paged_decode8(const PagedDecodeParams& p, int nwg, int D, int dt, int wr, hipStream_t st,
                                 KernelTimer* t);
 hipError_t launch_paged_combine(const PagedDecodeParams& p, int D, hipStream_t st, KernelTimer* t);
 hipError_t launch_page_score(const PageSelectParams& p, int D, int dt, hipStream_t st, KernelTimer* t);

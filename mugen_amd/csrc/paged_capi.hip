@@ -85,17 +85,21 @@ float* align256(void* p) { return reinterpret_cast<float*>((reinterpret_cast<uin
 
 // turns per position of rope_dim / 2 pairs: theta^(-2i/rope_dim) / (2 pi), for
 // factor > 1 with the YaRN correction of yarn_rope_freq (transformer.cpp:41-70;
-// beta_fast 32, beta_slow 1), in 64 bits
+// beta_fast 32, beta_slow 1), in 64 bits (the powers by repeated products in extended
+// precision: a pow() a pair took 3 us of a call)
 RopeTurns rope_turns(const mugen_attn_rope_params& r, int rope_dim) {
     RopeTurns out{};
     const double two_pi = 6.283185307179586476925286766559;
     const double theta = r.theta, dim = rope_dim;
-    for (int i = 0; i < rope_dim / 2; i++) {
-        double f = std::pow(theta, -2.0 * i / dim);
-        if (r.factor > 1.f) {
-            const double span = 2.0 * std::log(theta);
-            const double low = std::max(0.0, std::floor(dim * std::log(r.original_ctx / (32.0 * two_pi)) / span));
-            const double high = std::min(dim / 2 - 1, std::ceil(dim * std::log(r.original_ctx / two_pi) / span));
+    const bool yarn = r.factor > 1.f;
+    const double span = yarn ? 2.0 * std::log(theta) : 1.0;
+    const double low = yarn ? std::max(0.0, std::floor(dim * std::log(r.original_ctx / (32.0 * two_pi)) / span)) : 0.0;
+    const double high = yarn ? std::min(dim / 2 - 1, std::ceil(dim * std::log(r.original_ctx / two_pi) / span)) : 0.0;
+    const long double step = powl((long double)theta, -2.0L / rope_dim);
+    long double power = 1.0L;
+    for (int i = 0; i < rope_dim / 2; i++, power *= step) {
+        double f = (double)power;
+        if (yarn) {
             const double ramp = i < low ? 0.0 : i > high ? 1.0 : (i - low) / std::max(0.001, high - low);
             f = f * (1.0 - std::min(1.0, ramp)) + f / r.factor * std::min(1.0, ramp);
         }
@@ -176,7 +180,7 @@ namespace {
 struct DecodePlan {
     int chunk = 0;   // 0: planned by the kernels
     int splits = 1;  // the partials' stride
-    int nr = 1, nrb = 1;
+    int wr = 1, nrb = 1;  // row blocks of a workgroup, workgroups of a (range, kv head)
     int budget = 0;
     int64_t nwg = 0;
     size_t bytes = 0;
@@ -221,10 +225,10 @@ DecodePlan decode_plan(const mugen_attn_gqa_decode_paged_args* a, bool for_size)
     DecodePlan r;
     const mugen_attn_kv_pages& s = a->store;
     const int G = a->n_heads / s.n_kv_heads, rows = (a->pages ? 1 : a->q_len) * G;
-    if (!a->pages) r.nr = rows <= 16 ? 1 : rows <= 32 || s.head_dim == 256 ? 2 : 4;
-    r.nrb = (int)ceil_div(rows, 16 * r.nr);
+    r.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 && s.head_dim < 256 ? 3 : 4;
+    r.nrb = (int)ceil_div(rows, 16 * r.wr);
     const int64_t mult = (int64_t)s.n_kv_heads * r.nrb;
-    r.budget = s.head_dim == 256 || r.nr > 1 ? 256 : 512;
+    r.budget = s.head_dim == 256 || r.wr > 1 ? 256 : 512;
     const int64_t longest = longest_range(a);
     int64_t len = 1;
     for (int x = 0, R = a->seq_lens_host ? ranges_of(a) : 1; x < R; x++) len = std::max(len, range_len(a, x));
@@ -323,8 +327,8 @@ int decode_run(const mugen_attn_gqa_decode_paged_args* a, const DecodePlan& plan
     if (plan.nwg > INT32_MAX / 2 || (int64_t)p.B * p.q_len > 65535 * (int64_t)p.q_len || (int64_t)s.n_seq * a->q_len > 65535)
         return fail(MUGEN_ATTN_E_UNSUPPORTED, "gqa_decode_paged: too many sequences or work items");
     hipError_t e = s.page_bits == 8
-                       ? launch_paged_decode8(p, (int)plan.nwg, s.head_dim, s.dtype, plan.nr, st, active_timer())
-                       : launch_paged_decode16(p, (int)plan.nwg, s.head_dim, s.dtype, plan.nr, st, active_timer());
+                       ? launch_paged_decode8(p, (int)plan.nwg, s.head_dim, s.dtype, plan.wr, st, active_timer())
+                       : launch_paged_decode16(p, (int)plan.nwg, s.head_dim, s.dtype, plan.wr, st, active_timer());
     if (e == hipSuccess && plan.splits > 1) e = launch_paged_combine(p, s.head_dim, st, active_timer());
     return hip_status(e, "gqa_decode_paged launch");
 }

@@ -7,10 +7,13 @@
 //
 // Design (HBM-bound: each K and V byte is read once):
 //  * one workgroup = (context split, kv head, sequence, row block); its rows
-//    are (token, head of the group) pairs, up to NR * 16 of them served from
-//    one read of K and V (a verify step's tokens share it);
-//  * 4 waves; wave w takes the 32-token tiles w, w+4, ... of the split and
-//    loads the next tile while computing the current one.  A page holds whole
+//    are (token, head of the group) pairs, 16 to a wave.  WR waves side by side
+//    take WR * 16 rows of the same tiles (a verify step's tokens share one read of
+//    K and V from HBM, the others hit L1), WT of them the 32-token tiles t, t + WT,
+//    ... of the split; each loads the next tile while computing the current one.
+//    (One wave with up to 4 row blocks needs over 600 registers at head_dim 128
+//    and spilled: 5 tokens of 28 / 4 heads over 4 x 31k tokens took 160 us.)
+//    A page holds whole
 //    tiles, so a tile's address is one page id away: the ids (and the 8-bit
 //    scales) of 64 pages sit in one register across the lanes, read with
 //    v_readlane, the next 64 loaded ahead;
@@ -31,7 +34,7 @@
 //    weighted 0: 0 * inf is NaN.  Tiles that reach past the first query's last token
 //    are checked for values that are not finite; where one is met, each token's
 //    rows get their own product with the later rows zeroed;
-//  * the 4 waves merge (m, l, o) through LDS; with one split the result is
+//  * the WT waves of a row block merge (m, l, o) through LDS; with one split the result is
 //    stored, otherwise fp32 partials go to the workspace and the combine merges
 //    them.
 #pragma once
@@ -94,15 +97,17 @@ __device__ __forceinline__ int plan(const PagedDecodeParams& p) {
         [&](int j, int c, float rc) { return max(1, ceil_div_f(units(j), c, rc)); });
 }
 
-// two waves per SIMD where a wave's operands fit in half the registers
-template <int D, int DT, bool BITS8, int NR, bool LIST>
-constexpr int waves_per_eu() {
-    return D > 128 || NR > (BITS8 ? 2 : 1) ? 1 : 2;
+// waves that take a tile's row blocks side by side (WR), and tiles under way
+// (WT): 8 waves are what two to a SIMD hold, 4 at head_dim 256, where a wave's
+// operands need a whole SIMD's registers
+__host__ __device__ constexpr int tile_waves(int D, int WR) {
+    return D == 256 ? 4 / WR : WR <= 2 ? 4 : 2;
 }
 
-template <int D, int DT, bool BITS8, int NR, bool LIST>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves_per_eu<D, DT, BITS8, NR, LIST>()))) void
-paged_decode_kernel(PagedDecodeParams p) {
+template <int D, int DT, bool BITS8, int WR, bool LIST>
+__global__ __launch_bounds__(64 * WR * tile_waves(D, WR))
+    __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void paged_decode_kernel(PagedDecodeParams p) {
+    constexpr int WT = tile_waves(D, WR), NW = WR * WT, STEP = 32 * WT;
     constexpr int KK = D / 32;          // MFMA k-steps of S
     constexpr int KJ = D / 64;          // 16-byte loads of an 8-bit K row per lane
     constexpr int DB = D / 16;          // 16-dim blocks of O^T
@@ -112,9 +117,9 @@ paged_decode_kernel(PagedDecodeParams p) {
     constexpr int NP = p_terms<DT>();
     constexpr float kHeadroom = 8.f;
     constexpr int kNever = 0x3fffffff;  // a tile that no row sees
-    constexpr int STAGE = 4 * 32 * RB;
+    constexpr int STAGE = NW * 32 * RB;
     constexpr int OROW = D + 4;
-    constexpr int MERGE = 4 * 16 * OROW * 4 + 3 * 4 * 16 * 4 + 2 * 16 * 4;
+    constexpr int MERGE = NW * 16 * OROW * 4 + 3 * NW * 16 * 4 + WR * 2 * 16 * 4;
     __shared__ __attribute__((aligned(16))) char lds[STAGE > MERGE ? STAGE : MERGE];
 
     const int Hk = p.st.Hk, ps = p.st.p_shift, P = 1 << ps;
@@ -137,38 +142,31 @@ paged_decode_kernel(PagedDecodeParams p) {
     const int t_begin = s * chunk, t_end = min(t_begin + chunk, range);
     if (p.chunk == 0 && blockIdx.x == 0 && threadIdx.x == 0) *p.plan = chunk;  // for the merge
     if (p.num_splits > 1 && t_begin >= t_end) return;  // nothing to see: the merge skips it
-    const int G = p.G, first_row = rb * NR * 16, n_rows = (LIST ? 1 : len.n) * G;
-    if (first_row >= n_rows) return;  // rows of tokens that are not there
+    const int G = p.G, wg_row = rb * WR * 16, n_rows = (LIST ? 1 : len.n) * G;
+    if (wg_row >= n_rows) return;  // rows of tokens that are not there
+    const int wr = w % WR, wt = w / WR, first_row = wg_row + 16 * wr;
 
-    // the lane's rows 16 * rr + n: their queries, and how many tokens they see
-    u32x4_t qf[NR][KK];
-    int limit[NR], tok[NR];
-    int low = T;  // the first query's tokens: tiles below it are seen by every row
-#pragma unroll
-    for (int rr = 0; rr < NR; rr++) {
-        const int row = first_row + 16 * rr + n;
-        const int i = LIST ? i0 : row / G, h = LIST ? row : row - i * G;
-        const bool live = row < n_rows;
-        tok[rr] = live ? i : -1;
-        limit[rr] = live ? max(T - len.n + i + 1, 0) : 0;
-        const uint16_t* qp = p.q + (((int64_t)b * p.q_len + i) * p.H + kvh * G + h) * D;
+    // the lane's row first_row + n: its query, and how many tokens that sees
+    const int row = first_row + n;
+    const bool live = row < n_rows;
+    const int tok = LIST ? i0 : row / G;
+    const int limit = live ? max(T - len.n + tok + 1, 0) : 0;
+    u32x4_t qf[KK];
+    {
+        const uint16_t* qp = p.q + (((int64_t)b * p.q_len + tok) * p.H + kvh * G + (LIST ? row : row - tok * G)) * D;
 #pragma unroll
         for (int kk = 0; kk < KK; kk++)
-            qf[rr][kk] = live ? load16(qp + 64 * (kk >> 1) + 16 * g + 8 * (kk & 1)) : u32x4_t{0, 0, 0, 0};
+            qf[kk] = live ? load16(qp + 64 * (kk >> 1) + 16 * g + 8 * (kk & 1)) : u32x4_t{0, 0, 0, 0};
     }
-    const int tok_first = LIST ? i0 : first_row / G;
-    const int tok_last = LIST ? i0 : (min(first_row + NR * 16, n_rows) - 1) / G;
-    low = max(T - len.n + tok_first + 1, 0);
+    // the wave's first and last token; tiles below `low` are seen by all its rows
+    const int tok_first = LIST ? i0 : first_row / G, tok_last = LIST ? i0 : (min(first_row + 16, n_rows) - 1) / G;
+    const int low = first_row < n_rows ? max(T - len.n + tok_first + 1, 0) : 0;
+    const int t_first = first_row < n_rows ? t_begin + 32 * wt : t_end;  // (a wave without rows has no tiles)
 
-    f32x4_t o[NR][DB];  // lane (g, n): O[row 16 rr + n][16d + 4g + i]
-    float m_run[NR], l_part[NR];
+    f32x4_t o[DB];  // lane (g, n): O[row n][16d + 4g + i]
+    float m_run = kNegInf, l_part = 0.f;
 #pragma unroll
-    for (int rr = 0; rr < NR; rr++) {
-        m_run[rr] = kNegInf;
-        l_part[rr] = 0.f;
-#pragma unroll
-        for (int d = 0; d < DB; d++) o[rr][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int d = 0; d < DB; d++) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
     // ---- page ids: lane l holds page first_page + l of the split, physical
     // (-1: not there), logical (LIST), and the two exponents
@@ -182,7 +180,7 @@ paged_decode_kernel(PagedDecodeParams p) {
         uint32_t exps;
     };
     auto load_ids = [&](int page0) {
-        Ids x{-1, -1, 0};
+        Ids x{-1, -1, 0x0101};  // (exponents of a page that is not there: any that are finite)
         const int k = page0 + lane;
         if (k < end_page) {
             int lp = k;
@@ -204,7 +202,7 @@ paged_decode_kernel(PagedDecodeParams p) {
         }
         return x;
     };
-    Ids ids = load_ids(first_page), ids_next{-1, -1, 0};
+    Ids ids = load_ids(first_page), ids_next = ids;
     int ids_at = first_page;
     if (ids_at + 64 < end_page) ids_next = load_ids(ids_at + 64);
 
@@ -230,64 +228,60 @@ paged_decode_kernel(PagedDecodeParams p) {
     };
 
     // ---- softmax of one tile's scores (lane: 8 consecutive tokens of its
-    // rows), P as the B operand
-    auto softmax_tile = [&](f32x4_t (&sacc)[NR][2], int t0, float scale, u32x4_t (&pf)[NR][NP]) {
+    // rows), P as the B operand.  The maximum is taken of the raw scores (scale > 0)
+    // and the scale goes into the exponent's fma; only edge tiles are masked
+    auto softmax_tile = [&](f32x4_t (&sacc)[2], int t0, auto edge, float scale, u32x4_t (&pf)[NP]) {
+        float x[8];
 #pragma unroll
-        for (int rr = 0; rr < NR; rr++) {
-            float x[8];
-            float smax = kNegInf;
-            const int seen = limit[rr] - t0 - 8 * g;
+        for (int e = 0; e < 8; e++) x[e] = sacc[e >> 2][e & 3];
+        if constexpr (decltype(edge)::value) {
+            const int seen = limit - t0 - 8 * g;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = e < seen ? sacc[rr][e >> 2][e & 3] * scale : kNegInf;
-                x[e] = v;
-                smax = fmaxf(smax, v);
-            }
-            if (__any(smax > m_run[rr] + kHeadroom)) {  // re-base the rows (wave-uniform branch)
-                const float m_new = fmaxf(m_run[rr], max_x32(max_x16(smax)));
-                if (m_new > m_run[rr]) {
-                    const float alpha = fast_exp2(m_run[rr] - m_new);  // 0 while m_run = -inf
-                    l_part[rr] *= alpha;
-#pragma unroll
-                    for (int d = 0; d < DB; d++) o[rr][d] *= alpha;
-                    m_run[rr] = m_new;
-                }
-            }
-            const float nm = m_run[rr] == kNegInf ? 0.f : -m_run[rr];
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x[e] = fast_exp2(x[e] + nm);
-                sum += x[e];
-            }
-            l_part[rr] += sum;
-            split_p<DT, NP>(x, pf[rr]);
+            for (int e = 0; e < 8; e++) x[e] = e < seen ? x[e] : kNegInf;
         }
+        float smax = x[0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) smax = fmaxf(smax, x[e]);
+        smax *= scale;
+        if (__any(smax > m_run + kHeadroom)) {  // re-base the rows (wave-uniform branch)
+            const float m_new = fmaxf(m_run, max_x32(max_x16(smax)));
+            if (m_new > m_run) {
+                const float alpha = fast_exp2(m_run - m_new);  // 0 while m_run = -inf
+                l_part *= alpha;
+#pragma unroll
+                for (int d = 0; d < DB; d++) o[d] *= alpha;
+                m_run = m_new;
+            }
+        }
+        const float nm = m_run == kNegInf ? 0.f : -m_run;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            x[e] = fast_exp2(fmaf(x[e], scale, nm));
+            sum += x[e];
+        }
+        l_part += sum;
+        split_p<DT, NP>(x, pf);
     };
     // O^T += V^T.P^T, V^T blocks from vt(d)
-    auto product = [&](auto vt, u32x4_t (&pf)[NR][NP]) {
+    auto product = [&](auto vt, u32x4_t (&pf)[NP]) {
 #pragma unroll
         for (int d = 0; d < DB; d++) {
             const u32x4_t a = vt(d);
 #pragma unroll
-            for (int rr = 0; rr < NR; rr++)
-#pragma unroll
-                for (int t = 0; t < NP; t++) o[rr][d] = mfma16x16x32<DT>(a, pf[rr][t], o[rr][d]);
+            for (int t = 0; t < NP; t++) o[d] = mfma16x16x32<DT>(a, pf[t], o[d]);
         }
     };
     // the same for the rows of token i alone (a lane holds one row of O; the
     // others' weights are no zeros that would keep a NaN out)
-    auto product_of = [&](int i, auto vt, u32x4_t (&pf)[NR][NP]) {
+    auto product_of = [&](int i, auto vt, u32x4_t (&pf)[NP]) {
 #pragma unroll
         for (int d = 0; d < DB; d++) {
             const u32x4_t a = vt(d);
+            f32x4_t x = o[d];
 #pragma unroll
-            for (int rr = 0; rr < NR; rr++) {
-                f32x4_t x = o[rr][d];
-#pragma unroll
-                for (int t = 0; t < NP; t++) x = mfma16x16x32<DT>(a, pf[rr][t], x);
-                if (tok[rr] == i) o[rr][d] = x;
-            }
+            for (int t = 0; t < NP; t++) x = mfma16x16x32<DT>(a, pf[t], x);
+            if (tok == i) o[d] = x;
         }
     };
 
@@ -306,24 +300,20 @@ paged_decode_kernel(PagedDecodeParams p) {
             vq[x] = load16(vb + min(x * RPL + lane / (RB / 16), last) * stride + 8 * (lane % (RB / 16)));
     };
     char* stage = &lds[w * 32 * RB];
-    uint32_t st_off[VL], t_off[DB];
-#pragma unroll
-    for (int x = 0; x < VL; x++) {
+    auto st_off = [&](int x) {
         const int row = x * RPL + lane / (RB / 16), c = lane % (RB / 16);
-        st_off[x] = row * RB + ((c ^ swz<D>(row)) * 16);
-    }
+        return row * RB + ((c ^ swz<D>(row)) * 16);
+    };
     const int tr = 8 * g + (n >> 2);
-#pragma unroll
-    for (int d = 0; d < DB; d++)
-        t_off[d] = tr * RB + (((2 * d + ((n & 3) >> 1)) ^ swz<D>(tr)) * 16) + 8 * (n & 1);
+    auto t_off = [&](int d) { return tr * RB + (((2 * d + ((n & 3) >> 1)) ^ swz<D>(tr)) * 16) + 8 * (n & 1); };
     auto wave_sync = [] {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
     auto staged = [&](int d) {
-        const u32x2_t lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(stage + t_off[d]));
-        const u32x2_t hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(stage + t_off[d] + 4 * RB));
+        const u32x2_t lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(stage + t_off(d)));
+        const u32x2_t hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(stage + t_off(d) + 4 * RB));
         return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
     };
     // V rows from `seen` on zeroed
@@ -331,28 +321,26 @@ paged_decode_kernel(PagedDecodeParams p) {
 #pragma unroll
         for (int x = 0; x < VL; x++) {
             const bool in = x * RPL + lane / (RB / 16) < seen;
-            *reinterpret_cast<u32x4_t*>(stage + st_off[x]) = in ? vq[x] : u32x4_t{0, 0, 0, 0};
+            *reinterpret_cast<u32x4_t*>(stage + st_off(x)) = in ? vq[x] : u32x4_t{0, 0, 0, 0};
         }
     };
-    auto compute16 = [&](u32x4_t (&kq)[2][KK], u32x4_t (&vq)[VL], int t0) {
-        const bool edge = t0 + 32 > low;
-        if (!edge) {
+    auto compute16 = [&](u32x4_t (&kq)[2][KK], u32x4_t (&vq)[VL], int t0, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+        if constexpr (!EDGE) {
 #pragma unroll
-            for (int x = 0; x < VL; x++) *reinterpret_cast<u32x4_t*>(stage + st_off[x]) = vq[x];
+            for (int x = 0; x < VL; x++) *reinterpret_cast<u32x4_t*>(stage + st_off(x)) = vq[x];
         }
-        f32x4_t sacc[NR][2];
+        f32x4_t sacc[2];
 #pragma unroll
-        for (int rr = 0; rr < NR; rr++)
+        for (int nb = 0; nb < 2; nb++) {
+            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int nb = 0; nb < 2; nb++) {
-                f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kk = 0; kk < KK; kk++) acc = mfma16x16x32<DT>(kq[nb][kk], qf[rr][kk], acc);
-                sacc[rr][nb] = acc;
-            }
-        u32x4_t pf[NR][NP];
-        softmax_tile(sacc, t0, p.scale_log2, pf);
-        if (edge) {
+            for (int kk = 0; kk < KK; kk++) acc = mfma16x16x32<DT>(kq[nb][kk], qf[kk], acc);
+            sacc[nb] = acc;
+        }
+        u32x4_t pf[NP];
+        softmax_tile(sacc, t0, edge, p.scale_log2, pf);
+        if constexpr (EDGE) {
             bool bad = false;
 #pragma unroll
             for (int x = 0; x < VL; x++)
@@ -367,32 +355,40 @@ paged_decode_kernel(PagedDecodeParams p) {
                 }
                 return;
             }
-            stage_rows(vq, (LIST ? my_limit : T - len.n + tok_last + 1) - t0);
+            stage_rows(vq, T - len.n + tok_last + 1 - t0);
         }
         wave_sync();
         product(staged, pf);
         wave_sync();
     };
 
+    // ---- The tiles: first those that every row sees whole, the next one loading
+    // meanwhile (tiles of a page that is not there are passed over), then the last
+    // few, which some row sees in part: the range ascends, so they come last.
     if constexpr (!BITS8) {
         u32x4_t kf[2][KK], kn[2][KK], vf[VL], vn[VL];
-        auto load = [&](int t, u32x4_t (&kq)[2][KK], u32x4_t (&vq)[VL]) {
-            const Tile x = find_tile(t);
+        auto load = [&](const Tile& x, u32x4_t (&kq)[2][KK], u32x4_t (&vq)[VL]) {
             const int64_t at = ((((int64_t)max(x.phys, 0) * Hk + kvh) << ps) + x.off) * D;
             // tokens past the sequence are not read: the last one instead
             load16_tile(reinterpret_cast<const uint16_t*>(p.st.k) + at, reinterpret_cast<const uint16_t*>(p.st.v) + at, D,
                         min(31, max(T - 1 - x.t0, 0)), kq, vq);
-            return x.t0;
         };
-        int t = t_begin + 32 * w;
-        int t0 = kNever, t0_next = kNever;
-        if (t < t_end) t0 = load(t, kf, vf);
-        for (; t < t_end; t += 128) {
-            const bool more = t + 128 < t_end;
-            if (more) t0_next = load(t + 128, kn, vn);
-            compute16(kf, vf, t0);
+        int t = t_first;
+        Tile at{-1, 0, kNever, 0}, at_next = at;
+        if (t < t_end) {
+            at = find_tile(t);
+            load(at, kf, vf);
+        }
+        for (; t < t_end; t += STEP) {
+            if (at.phys >= 0 && at.t0 + 32 > low) break;
+            const bool more = t + STEP < t_end;
             if (more) {
-                t0 = t0_next;
+                at_next = find_tile(t + STEP);
+                load(at_next, kn, vn);
+            }
+            if (at.phys >= 0) compute16(kf, vf, at.t0, std::false_type{});
+            if (more) {
+                at = at_next;
 #pragma unroll
                 for (int nb = 0; nb < 2; nb++)
 #pragma unroll
@@ -401,13 +397,19 @@ paged_decode_kernel(PagedDecodeParams p) {
                 for (int x = 0; x < VL; x++) vf[x] = vn[x];
             }
         }
+        for (; t < t_end; t += STEP) {
+            if (at.phys >= 0) compute16(kf, vf, at.t0, std::true_type{});
+            if (t + STEP < t_end) {
+                at = find_tile(t + STEP);
+                load(at, kf, vf);
+            }
+        }
     } else {
         struct Raw {
             u32x4_t k[2][KJ];
             u32x2_t v[DB];
         };
-        auto load = [&](int t, Raw& x) {
-            const Tile at = find_tile(t);
+        auto load = [&](const Tile& at, Raw& x) {
             const int64_t base = ((((int64_t)max(at.phys, 0) * Hk + kvh) << ps) + at.off) * D;
             const uint8_t* kb = p.st.k + base;
             const uint8_t* vb = p.st.v + base;
@@ -417,7 +419,6 @@ paged_decode_kernel(PagedDecodeParams p) {
                 for (int c = 0; c < KJ; c++) x.k[nb][c] = load16(kb + (kr0 + 4 * nb) * D + 64 * c + 16 * g);
 #pragma unroll
             for (int d = 0; d < DB; d++) x.v[d] = load8(vb + (16 * d + n) * 32 + 8 * g);
-            return at;
         };
         // V codes of tokens from `seen` on zeroed (the lane's tokens 8g .. 8g+7)
         auto keep = [&](u32x2_t v, int seen) {
@@ -425,9 +426,9 @@ paged_decode_kernel(PagedDecodeParams p) {
             const uint64_t mask = k >= 8 ? ~0ull : (1ull << (8 * k)) - 1;
             return u32x2_t{v[0] & (uint32_t)mask, v[1] & (uint32_t)(mask >> 32)};
         };
-        auto compute8 = [&](Raw& x, const Tile& at) {
+        auto compute8 = [&](Raw& x, const Tile& at, auto edge) {
             const float ks = exp_scale(at.exps & 0xffu) * p.scale_log2, vs = exp_scale((at.exps >> 8) & 0xffu);
-            f32x4_t sacc[NR][2];
+            f32x4_t sacc[2];
 #pragma unroll
             for (int nb = 0; nb < 2; nb++) {
                 u32x4_t kf[KK];
@@ -436,21 +437,18 @@ paged_decode_kernel(PagedDecodeParams p) {
                     kf[2 * c] = cvt8_fp8<DT>(x.k[nb][c][0], x.k[nb][c][1], 1.0f);
                     kf[2 * c + 1] = cvt8_fp8<DT>(x.k[nb][c][2], x.k[nb][c][3], 1.0f);
                 }
+                f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int rr = 0; rr < NR; rr++) {
-                    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int kk = 0; kk < KK; kk++) acc = mfma16x16x32<DT>(kf[kk], qf[rr][kk], acc);
-                    sacc[rr][nb] = acc;
-                }
+                for (int kk = 0; kk < KK; kk++) acc = mfma16x16x32<DT>(kf[kk], qf[kk], acc);
+                sacc[nb] = acc;
             }
-            u32x4_t pf[NR][NP];
-            softmax_tile(sacc, at.t0, ks, pf);
-            if (at.t0 + 32 > low) {
+            u32x4_t pf[NP];
+            softmax_tile(sacc, at.t0, edge, ks, pf);
+            if constexpr (decltype(edge)::value) {
                 bool bad = false;
 #pragma unroll
                 for (int d = 0; d < DB; d++) bad |= bad8(x.v[d][0]) | bad8(x.v[d][1]);
-                if (__any(bad)) {  // (a page that is not there: nothing seen, all zero)
+                if (__any(bad)) {
                     for (int i = tok_first; i <= tok_last; i++) {
                         const int seen = T - len.n + i + 1 - at.t0;
                         product_of(i, [&](int d) {
@@ -463,20 +461,34 @@ paged_decode_kernel(PagedDecodeParams p) {
             }
             product([&](int d) { return cvt8_fp8<DT>(x.v[d][0], x.v[d][1], vs); }, pf);
         };
-        // tiles in whole pages; the ring's page (dense: from token whole * P on;
-        // LIST: the last valid entry, met as a page that is not there) after them
+        // tiles in whole pages; the open page's, in the ring (dense: from token
+        // whole * P on; LIST: the last valid entry, here a page that is not there) after them
         const int end8 = LIST ? t_end : min(t_end, whole << ps);
-        int t = t_begin + 32 * w;
+        int t = t_first;
         Raw cur, nxt;
-        Tile at{-1, 0, kNever, 0}, at_next{-1, 0, kNever, 0};
-        if (t < end8) at = load(t, cur);
-        for (; t < end8; t += 128) {
-            const bool more = t + 128 < end8;
-            if (more) at_next = load(t + 128, nxt);
-            compute8(cur, at);
+        Tile at{-1, 0, kNever, 0x0101}, at_next = at;
+        if (t < end8) {
+            at = find_tile(t);
+            load(at, cur);
+        }
+        for (; t < end8; t += STEP) {
+            if (at.phys >= 0 && at.t0 + 32 > low) break;
+            const bool more = t + STEP < end8;
+            if (more) {
+                at_next = find_tile(t + STEP);
+                load(at_next, nxt);
+            }
+            if (at.phys >= 0) compute8(cur, at, std::false_type{});
             if (more) {
                 cur = nxt;
                 at = at_next;
+            }
+        }
+        for (; t < end8; t += STEP) {
+            if (at.phys >= 0) compute8(cur, at, std::true_type{});
+            if (t + STEP < end8) {
+                at = find_tile(t + STEP);
+                load(at, cur);
             }
         }
         // ---- the open page
@@ -493,101 +505,104 @@ paged_decode_kernel(PagedDecodeParams p) {
         if (open >= first_page && open < end_page) {
             // this wave's tiles of the page inside the split
             const int lo = max(open << ps, t_begin), hi = min((open + 1) << ps, t_end);
-            int tt = t_begin + 32 * w;
-            if (tt < lo) tt += (lo - tt + 127) / 128 * 128;
-            for (; tt < hi; tt += 128) {
+            int tt = t_first;
+            if (tt < lo) tt += (lo - tt + STEP - 1) / STEP * STEP;
+            for (; tt < hi; tt += STEP) {
                 const int t0 = (whole << ps) + (tt & (P - 1));  // its first token
                 if (t0 >= T) break;
                 const int64_t ring_at = b * p.st.tail_stride + ((int64_t)(t0 & (p.st.ring - 1)) * Hk + kvh) * D;
                 u32x4_t kq[2][KK], vq[VL];
                 load16_tile(p.st.tail_k + ring_at, p.st.tail_v + ring_at, Hk * D, min(31, T - 1 - t0), kq, vq);
-                compute16(kq, vq, t0);
+                compute16(kq, vq, t0, std::true_type{});
             }
         }
     }
 
-    // ---- merge the 4 waves' (m, l, O) per row through LDS, a row block at a time
-    float* o_lds = reinterpret_cast<float*>(&lds[0]);  // [4][16][OROW]
-    float* m_lds = o_lds + 4 * 16 * OROW;              // [4][16]
-    float* l_lds = m_lds + 4 * 16;
-    float* f_lds = l_lds + 4 * 16;                     // [4][16]: the waves' factors
-    float* ml_out = f_lds + 4 * 16;                    // [16][2]: the row's (M, L)
+    // ---- merge the WT waves' (m, l, O) of each row through LDS
+    float* o_lds = reinterpret_cast<float*>(&lds[0]);  // [NW][16][OROW]
+    float* m_lds = o_lds + NW * 16 * OROW;             // [NW][16]
+    float* l_lds = m_lds + NW * 16;
+    float* f_lds = l_lds + NW * 16;                    // [NW][16]: the waves' factors
+    float* ml_out = f_lds + NW * 16;                   // [WR][16][2]: the row's (M, L)
+    const float l = sum_x32(sum_x16(l_part));
+    __syncthreads();
 #pragma unroll
-    for (int rr = 0; rr < NR; rr++) {
-        if (first_row + 16 * rr >= n_rows) break;  // (uniform)
-        const float l = sum_x32(sum_x16(l_part[rr]));
-        __syncthreads();
+    for (int d = 0; d < DB; d++) *reinterpret_cast<f32x4_t*>(&o_lds[(w * 16 + n) * OROW + 16 * d + 4 * g]) = o[d];
+    if (g == 0) {
+        // (a NaN sum behind a maximum that no number set still counts)
+        m_lds[w * 16 + n] = l != l && m_run == kNegInf ? 0.f : m_run;
+        l_lds[w * 16 + n] = l;
+    }
+    __syncthreads();
+    if (threadIdx.x < 16 * WR) {
+        const int h = threadIdx.x;  // row of the workgroup: wave x * WR + h / 16, its row h % 16
+        auto at = [&](int x) { return (x * WR + (h >> 4)) * 16 + (h & 15); };
+        float M = kNegInf;
 #pragma unroll
-        for (int d = 0; d < DB; d++)
-            *reinterpret_cast<f32x4_t*>(&o_lds[(w * 16 + n) * OROW + 16 * d + 4 * g]) = o[rr][d];
-        if (g == 0) {
-            // (a NaN sum behind a maximum that no number set still counts)
-            m_lds[w * 16 + n] = l != l && m_run[rr] == kNegInf ? 0.f : m_run[rr];
-            l_lds[w * 16 + n] = l;
+        for (int x = 0; x < WT; x++) M = fmaxf(M, m_lds[at(x)]);
+        float f[WT], L = 0.f;
+#pragma unroll
+        for (int x = 0; x < WT; x++) {
+            const float mw = m_lds[at(x)];
+            f[x] = mw == kNegInf ? 0.f : fast_exp2(mw - M);
+            L += f[x] * l_lds[at(x)];
         }
-        __syncthreads();
-        if (threadIdx.x < 16) {
-            const int h = threadIdx.x;
-            float M = kNegInf;
+        const float c = p.num_splits == 1 ? (L > 0.f ? 1.f / L : L == L ? 0.f : L) : 1.f;
 #pragma unroll
-            for (int x = 0; x < 4; x++) M = fmaxf(M, m_lds[x * 16 + h]);
-            float f[4], L = 0.f;
+        for (int x = 0; x < WT; x++) f_lds[at(x)] = f[x] * c;
+        ml_out[2 * h] = M;
+        ml_out[2 * h + 1] = L;
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < WR * 16 * D; idx += 64 * NW) {
+        const int h = idx / D, d = idx - h * D, r2 = wg_row + h;
+        if (r2 >= n_rows) break;
+        const int i = LIST ? i0 : r2 / G, hh = LIST ? r2 : r2 - i * G;
+        float O = 0.f;
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const float mw = m_lds[x * 16 + h];
-                f[x] = mw == kNegInf ? 0.f : fast_exp2(mw - M);
-                L += f[x] * l_lds[x * 16 + h];
-            }
-            const float c = p.num_splits == 1 ? (L > 0.f ? 1.f / L : L == L ? 0.f : L) : 1.f;
-#pragma unroll
-            for (int x = 0; x < 4; x++) f_lds[x * 16 + h] = f[x] * c;
-            ml_out[2 * h] = M;
-            ml_out[2 * h + 1] = L;
+        for (int x = 0; x < WT; x++) {
+            const int at = (x * WR + (h >> 4)) * 16 + (h & 15);
+            const float f = f_lds[at];
+            O += f == 0.f ? 0.f : f * o_lds[at * OROW + d];
         }
-        __syncthreads();
-        for (int idx = threadIdx.x; idx < 16 * D; idx += 256) {
-            const int h = idx / D, d = idx - h * D, row = first_row + 16 * rr + h;
-            if (row >= n_rows) break;
-            const int i = LIST ? i0 : row / G, hh = LIST ? row : row - i * G;
-            float O = 0.f;
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const float f = f_lds[x * 16 + h];
-                O += f == 0.f ? 0.f : f * o_lds[(x * 16 + h) * OROW + d];
-            }
-            const int64_t orow = ((int64_t)b * p.q_len + i) * p.H + kvh * G + hh;
-            if (p.num_splits == 1) {
-                if (p.out_dt == DT_F32) store_out<DT_F32>(p.out, orow * D + d, O);
-                else if (p.out_dt == DT_F16) store_out<DT_F16>(p.out, orow * D + d, O);
-                else store_out<DT_BF16>(p.out, orow * D + d, O);
-            } else {
-                const int64_t slot = orow * p.num_splits + s;
-                p.ws_o[slot * D + d] = O;
-                if (d == 0) {
-                    p.ws_ml[slot * 2] = ml_out[2 * h];
-                    p.ws_ml[slot * 2 + 1] = ml_out[2 * h + 1];
-                }
+        const int64_t orow = ((int64_t)b * p.q_len + i) * p.H + kvh * G + hh;
+        if (p.num_splits == 1) {
+            if (p.out_dt == DT_F32) store_out<DT_F32>(p.out, orow * D + d, O);
+            else if (p.out_dt == DT_F16) store_out<DT_F16>(p.out, orow * D + d, O);
+            else store_out<DT_BF16>(p.out, orow * D + d, O);
+        } else {
+            const int64_t slot = orow * p.num_splits + s;
+            p.ws_o[slot * D + d] = O;
+            if (d == 0) {
+                p.ws_ml[slot * 2] = ml_out[2 * h];
+                p.ws_ml[slot * 2 + 1] = ml_out[2 * h + 1];
             }
         }
     }
 }
 
 template <int D, int DT, bool BITS8>
-hipError_t launch_rows(const PagedDecodeParams& p, int nwg, int nr, hipStream_t st, KernelTimer* t) {
-    const dim3 grid(nwg), block(256);
-    if (p.sel) return launch_k(t, "gqa_decode_paged", paged_decode_kernel<D, DT, BITS8, 1, true>, grid, block, st, p);
-    if (nr == 1) return launch_k(t, "gqa_decode_paged", paged_decode_kernel<D, DT, BITS8, 1, false>, grid, block, st, p);
-    if constexpr (D <= 128)
-        if (nr == 4) return launch_k(t, "gqa_decode_paged", paged_decode_kernel<D, DT, BITS8, 4, false>, grid, block, st, p);
-    return launch_k(t, "gqa_decode_paged", paged_decode_kernel<D, DT, BITS8, 2, false>, grid, block, st, p);
+hipError_t launch_rows(const PagedDecodeParams& p, int nwg, int wr, hipStream_t st, KernelTimer* t) {
+    auto go = [&](auto r, auto list) {
+        constexpr int WR = decltype(r)::value;
+        return launch_k(t, "gqa_decode_paged", paged_decode_kernel<D, DT, BITS8, WR, decltype(list)::value>, dim3(nwg),
+                        dim3(64 * WR * tile_waves(D, WR)), st, p);
+    };
+    if (p.sel) return go(std::integral_constant<int, 1>{}, std::true_type{});
+    if (wr == 1) return go(std::integral_constant<int, 1>{}, std::false_type{});
+    if (wr == 2) return go(std::integral_constant<int, 2>{}, std::false_type{});
+    if constexpr (D < 256) {  // (3 does not divide a CU's 4 waves there)
+        if (wr == 3) return go(std::integral_constant<int, 3>{}, std::false_type{});
+    }
+    return go(std::integral_constant<int, 4>{}, std::false_type{});
 }
 
 template <bool BITS8>
-hipError_t launch_decode(const PagedDecodeParams& p, int nwg, int D, int dt, int nr, hipStream_t st, KernelTimer* t) {
+hipError_t launch_decode(const PagedDecodeParams& p, int nwg, int D, int dt, int wr, hipStream_t st, KernelTimer* t) {
     auto by_dt = [&](auto d) {
         constexpr int DD = decltype(d)::value;
-        return dt == DT_F16 ? launch_rows<DD, DT_F16, BITS8>(p, nwg, nr, st, t)
-                            : launch_rows<DD, DT_BF16, BITS8>(p, nwg, nr, st, t);
+        return dt == DT_F16 ? launch_rows<DD, DT_F16, BITS8>(p, nwg, wr, st, t)
+                            : launch_rows<DD, DT_BF16, BITS8>(p, nwg, wr, st, t);
     };
     if (D == 256) return by_dt(std::integral_constant<int, 256>{});
     if (D == 128) return by_dt(std::integral_constant<int, 128>{});

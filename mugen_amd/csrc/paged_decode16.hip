@@ -8,7 +8,7 @@ namespace mugen_attn {
 // lane s holds split s's (m, l), the first partials are in flight meanwhile
 template <int D, bool LIST>
 __global__ __launch_bounds__(64) void paged_combine_kernel(PagedDecodeParams p) {
-    constexpr int kPre = 16;
+    constexpr int kPre = 32;
     __shared__ float f_lds[64];
     const int h = blockIdx.x, d = blockIdx.z * 64 + threadIdx.x, lane = threadIdx.x;
     const int b = (int)blockIdx.y / p.q_len, i = (int)blockIdx.y - b * p.q_len;
@@ -68,9 +68,9 @@ hipError_t launch_paged_combine(const PagedDecodeParams& p, int D, hipStream_t s
     return launch_combine_d<64>(p, st, t);
 }
 
-hipError_t launch_paged_decode16(const PagedDecodeParams& p, int nwg, int D, int dt, int nr, hipStream_t st,
+hipError_t launch_paged_decode16(const PagedDecodeParams& p, int nwg, int D, int dt, int wr, hipStream_t st,
                                  KernelTimer* t) {
-    return paged::launch_decode<false>(p, nwg, D, dt, nr, st, t);
+    return paged::launch_decode<false>(p, nwg, D, dt, wr, st, t);
 }
 
 }  // namespace mugen_attn

@@ -4,9 +4,9 @@
 
 namespace mugen_attn {
 
-hipError_t launch_paged_decode8(const PagedDecodeParams& p, int nwg, int D, int dt, int nr, hipStream_t st,
+hipError_t launch_paged_decode8(const PagedDecodeParams& p, int nwg, int D, int dt, int wr, hipStream_t st,
                                 KernelTimer* t) {
-    return paged::launch_decode<true>(p, nwg, D, dt, nr, st, t);
+    return paged::launch_decode<true>(p, nwg, D, dt, wr, st, t);
 }
 
 }  // namespace mugen_attn

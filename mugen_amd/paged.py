@@ -10,12 +10,13 @@ holds the memory; the work is in libmugen_attn.so.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
 import torch
 
 from . import _capi
-from .attention import _dt, _host_lens, _need_cuda, _ptr, _rope, _stream
+from .attention import _dt, _need_cuda
 
 
 def _data(t: torch.Tensor | None):
@@ -26,18 +27,62 @@ def _bytes(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.numel() * t.element_size()
 
 
-def _lens(t: torch.Tensor | None, n_seq: int, name: str):
-    if t is not None and (t.dtype != torch.int32 or t.numel() != n_seq or not t.is_cuda or not t.is_contiguous()):
-        raise ValueError(f"{name} must be a contiguous int32 device tensor [n_seq]")
-    return _data(t)
+# The calls run once per layer and step, and a decode step's take a few
+# microseconds: their arguments are packed in one go behind the store's bytes (a
+# struct by fields took 5 us more), and the library's functions take the bytes.
+def _packer(cls) -> struct.Struct:
+    """The fields of an argument struct behind its store, as the C compiler lays them out."""
+    code = {ctypes.c_void_p: "P", ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_float: "f"}
+    fmt = "".join(code[t] if t in code else "".join(code[u] for _, u in t._fields_) for _, t in cls._fields_[1:])
+    fmt = "@" + fmt
+    size, want = struct.calcsize(fmt), ctypes.sizeof(cls) - ctypes.sizeof(_capi.KvPages)
+    return struct.Struct(fmt + f"{want - size}x")
 
 
-def _token_stride(t: torch.Tensor, name: str) -> int:
+_APPEND, _DECODE, _SELECT, _PREFILL = (_packer(c) for c in (
+    _capi.KvPagedAppendArgs, _capi.GqaDecodePagedArgs, _capi.PageSelectArgs, _capi.GqaPrefillPagedArgs))
+
+
+class _Calls:
+    """The library's functions, taking packed arguments."""
+
+    def __init__(self):
+        L = _capi.lib()
+        vp, size = ctypes.c_void_p, ctypes.c_size_t
+
+        def fn(name, args, res=ctypes.c_int):
+            f = L["mugen_attn_" + name]  # (a function object of its own)
+            f.argtypes, f.restype = args, res
+            return f
+
+        self.append = fn("kv_paged_append", [vp, vp])
+        for name in ("gqa_decode_paged", "page_select", "gqa_prefill_paged"):
+            setattr(self, name, fn(name, [vp, vp, size, vp]))
+            setattr(self, name + "_size", fn(name + "_workspace_size", [vp], size))
+
+
+_calls: _Calls | None = None
+
+
+def _library() -> _Calls:
+    global _calls
+    if _calls is None:
+        _calls = _Calls()
+    return _calls
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", lambda: -1)
+_i32 = torch.int32
+
+
+def _token_stride(t: torch.Tensor, shape, name: str) -> int:
     """Elements between consecutive tokens of [n_seq, n_new, heads, head_dim],
     a slice of a fused projection or contiguous."""
-    B, n, H, D = t.shape
-    row = t.stride(1) if n > 1 else t.stride(0) if B > 1 else H * D
-    if t.stride(3) != 1 or (H > 1 and t.stride(2) != D) or (B > 1 and n > 1 and t.stride(0) != n * row) or row < H * D:
+    B, n, H, D = shape
+    s0, s1, s2, s3 = t.stride()
+    row = s1 if n > 1 else s0 if B > 1 else H * D
+    if s3 != 1 or (H > 1 and s2 != D) or (B > 1 and n > 1 and s0 != n * row) or row < H * D:
         raise ValueError(f"{name} must hold each token's heads together, tokens evenly apart")
     return row
 
@@ -97,22 +142,54 @@ class PagedStore:
         if bits8:
             s.ring, s.tail_seq_stride = tail_k.shape[1], tail_k.shape[1] * Hk * D
         s.n_kv_heads, s.head_dim, s.max_seq_len, s.dtype = Hk, D, int(max_seq_len), _dt(self.dtype)
-        # the calls' arguments start as copies of these
-        self._blank = {}
-        for cls in (_capi.KvPagedAppendArgs, _capi.GqaDecodePagedArgs, _capi.PageSelectArgs, _capi.GqaPrefillPagedArgs):
-            a = cls()
-            a.store = s
-            self._blank[cls] = bytes(a)
+        self._store = bytes(s)
+        self._index = k_pages.get_device()
+        self._dt16 = s.dtype
 
-    def _args(self, cls):
-        return cls.from_buffer_copy(self._blank[cls])
+    def _call(self, fn, *args):
+        """fn(*args, stream): torch's current stream of the store's device."""
+        if _current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return fn(*args, _raw_stream(self._index))
+        return fn(*args, _raw_stream(self._index))
 
-    def _heads(self, t: torch.Tensor, name: str, heads: int | None = None):
-        if t.dim() != 4 or t.shape[0] != self.n_seq or t.shape[3] != self.head_dim or t.dtype != self.dtype or \
-                (heads is not None and t.shape[2] != heads):
+    def _run(self, name: str, args: bytes, workspace: torch.Tensor | None):
+        """A call with a workspace: the given one, or one of the size asked for."""
+        lib = _library()
+        fn = getattr(lib, name)
+        if workspace is not None:
+            if workspace.get_device() != self._index or not workspace.is_contiguous():
+                raise ValueError("workspace must be a contiguous tensor on the store's device")
+            rc = self._call(fn, args, workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        else:
+            rc = self._call(fn, args, None, 0)
+            if rc == _capi.E_WORKSPACE:
+                n = getattr(lib, name + "_size")(args)
+                workspace = torch.empty(n, dtype=torch.uint8, device=self.device)
+                rc = self._call(fn, args, workspace.data_ptr(), n)
+        if rc:
+            _capi.check(rc)
+
+    def _heads(self, t: torch.Tensor, name: str):
+        """Shape of a [n_seq, tokens, heads, head_dim] tensor of the store's kind."""
+        shape = t.shape
+        if len(shape) != 4 or shape[0] != self.n_seq or shape[3] != self.head_dim or t.dtype is not self.dtype:
             raise ValueError(f"{name} must be [n_seq, tokens, heads, head_dim] in the store's dtype")
-        if not t.is_cuda:
-            raise ValueError("mugen_amd operators take device tensors (no CPU path)")
+        if t.get_device() != self._index:
+            raise ValueError(f"{name} must be on the store's device (no CPU path)")
+        return shape
+
+    def _lens(self, t: torch.Tensor | None, name: str) -> int:
+        if t is None:
+            return 0
+        if t.dtype is not _i32 or t.numel() != self.n_seq or t.get_device() != self._index or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor [n_seq] on the store's device")
+        return t.data_ptr()
+
+    def _like(self, out: torch.Tensor, shape, name: str, dtype=None):
+        if out.shape != shape or not out.is_contiguous() or out.get_device() != self._index or \
+                (dtype is not None and out.dtype is not dtype):
+            raise ValueError(f"{name} must be a contiguous {'' if dtype is None else dtype} tensor {tuple(shape)} on the store's device")
 
     # ------------------------------------------------------------- append
 
@@ -126,31 +203,31 @@ class PagedStore:
         q_out (returned).  rope: (theta, factor, original_ctx), None for no
         rotation; rope_dim: the rotated dims (default head_dim).  new_lens: tokens
         each sequence gets (default n_new); rows behind them are not touched."""
-        self._heads(k_new, "k_new", self.n_kv_heads)
-        self._heads(v_new, "v_new", self.n_kv_heads)
-        if k_new.shape != v_new.shape:
-            raise ValueError("k_new and v_new must have the same shape")
-        a = self._args(_capi.KvPagedAppendArgs)
-        a.n_new = n_new = k_new.shape[1]
+        shape = self._heads(k_new, "k_new")
+        if shape[2] != self.n_kv_heads or self._heads(v_new, "v_new") != shape:
+            raise ValueError("k_new and v_new must be [n_seq, n_new, n_kv_heads, head_dim]")
+        n_new = shape[1]
         if n_new == 0:
             return q_out
-        a.k_new, a.v_new = k_new.data_ptr(), v_new.data_ptr()
-        a.k_stride, a.v_stride = _token_stride(k_new, "k_new"), _token_stride(v_new, "v_new")
+        qp = qo = q_stride = H = 0
         if q is not None:
-            self._heads(q, "q")
-            if q.shape[1] != n_new:
+            qs = self._heads(q, "q")
+            if qs[1] != n_new:
                 raise ValueError("q must have as many tokens as k_new")
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            elif q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous() or not q_out.is_cuda:
-                raise ValueError("q_out must be a contiguous device tensor like q")
-            a.q, a.q_out, a.n_heads, a.q_stride = q.data_ptr(), q_out.data_ptr(), q.shape[2], _token_stride(q, "q")
-        a.seq_lens = _lens(seq_lens, self.n_seq, "seq_lens")
-        a.new_lens = _lens(new_lens, self.n_seq, "new_lens")
-        a.seq_lens_out = _lens(seq_lens_out, self.n_seq, "seq_lens_out")
-        if rope is not None:
-            a.rope, a.rope_dim = _rope(rope), self.head_dim if rope_dim is None else int(rope_dim)
-        _capi.check(_capi.lib().mugen_attn_kv_paged_append(ctypes.byref(a), _stream(self.device)))
+                q_out = torch.empty(qs, dtype=q.dtype, device=q.device)
+            else:
+                self._like(q_out, qs, "q_out", self.dtype)
+            qp, qo, q_stride, H = q.data_ptr(), q_out.data_ptr(), _token_stride(q, qs, "q"), qs[2]
+        theta, factor, ctx = (0.0, 0.0, 0) if rope is None else rope
+        dim = 0 if rope is None else self.head_dim if rope_dim is None else int(rope_dim)
+        args = self._store + _APPEND.pack(
+            k_new.data_ptr(), v_new.data_ptr(), qp, qo, self._lens(seq_lens, "seq_lens"), self._lens(new_lens, "new_lens"),
+            self._lens(seq_lens_out, "seq_lens_out"), _token_stride(k_new, shape, "k_new"),
+            _token_stride(v_new, shape, "v_new"), q_stride, n_new, H, dim, theta, factor, ctx)
+        rc = self._call(_library().append, args)
+        if rc:
+            _capi.check(rc)
         return q_out
 
     # ------------------------------------------------------------- attention
@@ -165,54 +242,44 @@ class PagedStore:
         behind them are not touched.  pages: int32 [n_seq, q_len, n_kv_heads,
         n_select] from select_pages, the only pages each query reads.
         seq_lens_host: optional host copy, balances the context splits."""
-        self._heads(q, "q")
+        shape = self._heads(q, "q")
         if not q.is_contiguous():
             raise ValueError("mugen_amd operators take contiguous tensors")
-        B, L, H, D = q.shape
         if out is None:
-            out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
-        elif out.shape != q.shape or not out.is_contiguous() or not out.is_cuda:
-            raise ValueError("out must be a contiguous device tensor like q")
-        a = self._args(_capi.GqaDecodePagedArgs)
-        a.q, a.out = q.data_ptr(), out.data_ptr()
-        a.seq_lens, a.q_lens = _lens(seq_lens, B, "seq_lens"), _lens(q_lens, B, "q_lens")
+            out = torch.empty(shape, dtype=out_dtype or q.dtype, device=q.device)
+        else:
+            self._like(out, shape, "out")
+        listed = n_select = 0
         if pages is not None:
-            if pages.dtype != torch.int32 or not pages.is_cuda or not pages.is_contiguous() or \
-                    pages.shape[:3] != (B, L, self.n_kv_heads):
-                raise ValueError("pages must be a contiguous int32 device tensor [n_seq, q_len, n_kv_heads, n_select]")
-            a.pages, a.n_select = pages.data_ptr(), pages.shape[3]
-        a.q_len, a.n_heads, a.num_splits, a.scale, a.out_dtype = L, H, int(num_splits), float(scale), _dt(out.dtype)
-        hl = _host_lens(seq_lens_host)
-        if hl is not None:
-            if hl.size != B:
+            n_select = pages.shape[-1]
+            self._like(pages, (*shape[:2], self.n_kv_heads, n_select), "pages", _i32)
+            listed = pages.data_ptr()
+        host = 0
+        if seq_lens_host is not None:
+            seq_lens_host = np.ascontiguousarray(seq_lens_host, np.int32)
+            if seq_lens_host.size != self.n_seq:
                 raise ValueError("seq_lens_host must have one entry per sequence")
-            a.seq_lens_host = hl.ctypes.data
-        L_ = _capi.lib()
-        n = _bytes(workspace)
-        rc = L_.mugen_attn_gqa_decode_paged(ctypes.byref(a), _ptr(workspace), n, _stream(self.device))
-        if rc == _capi.E_WORKSPACE and workspace is None:
-            n = L_.mugen_attn_gqa_decode_paged_workspace_size(ctypes.byref(a))
-            workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
-            rc = L_.mugen_attn_gqa_decode_paged(ctypes.byref(a), _ptr(workspace), n, _stream(self.device))
-        _capi.check(rc)
+            host = seq_lens_host.__array_interface__["data"][0]
+        args = self._store + _DECODE.pack(
+            q.data_ptr(), out.data_ptr(), self._lens(seq_lens, "seq_lens"), self._lens(q_lens, "q_lens"), listed, n_select,
+            shape[1], shape[2], num_splits, scale, self._dt16 if out.dtype is self.dtype else _dt(out.dtype), host)
+        self._run("gqa_decode_paged", args, workspace)
         return out
 
     def attention_workspace(self, q_len: int, n_heads: int, *, n_select: int = 0) -> torch.Tensor:
         """A workspace for every attention call of this shape, whatever its
         lengths (and select_pages', with n_select; the two may share it on one
         stream)."""
-        L = _capi.lib()
-        a = self._args(_capi.GqaDecodePagedArgs)
-        a.q = a.out = a.seq_lens = 16  # placeholders: only the shape matters for the size
-        a.q_len, a.n_heads, a.out_dtype = q_len, n_heads, _dt(self.dtype)
-        need = L.mugen_attn_gqa_decode_paged_workspace_size(ctypes.byref(a))
+        lib = _library()
+
+        def size(pages, n):  # (placeholder pointers: only the shape matters for the size)
+            return lib.gqa_decode_paged_size(self._store + _DECODE.pack(16, 16, 16, 0, pages, n, q_len, n_heads, 0, 0.0,
+                                                                        self._dt16, 0))
+
+        need = size(0, 0)
         if n_select:
-            a.pages, a.n_select = 16, n_select
-            need = max(need, L.mugen_attn_gqa_decode_paged_workspace_size(ctypes.byref(a)))
-            s = self._args(_capi.PageSelectArgs)
-            s.q = s.pages = s.seq_lens = 16
-            s.q_len, s.n_heads, s.n_select, s.n_first, s.n_last = q_len, n_heads, n_select, 0, 1
-            need = max(need, L.mugen_attn_page_select_workspace_size(ctypes.byref(s)))
+            need = max(need, size(16, n_select), lib.page_select_size(
+                self._store + _SELECT.pack(16, 16, 16, 0, q_len, n_heads, n_select, 0, 1)))
         return torch.empty(need, dtype=torch.uint8, device=self.device)
 
     def select_pages(self, q: torch.Tensor, seq_lens: torch.Tensor, n_select: int, *, first: int = 1, last: int = 2,
@@ -222,66 +289,45 @@ class PagedStore:
         ranges give: int32 [n_seq, q_len, n_kv_heads, n_select], ascending, -1
         behind them.  The first `first` and the newest `last` pages are always
         among them."""
-        self._heads(q, "q")
+        qs = self._heads(q, "q")
         if not q.is_contiguous():
             raise ValueError("mugen_amd operators take contiguous tensors")
-        B, L, H, D = q.shape
-        shape = (B, L, self.n_kv_heads, int(n_select))
+        shape = (qs[0], qs[1], self.n_kv_heads, n_select)
         if out is None:
-            out = torch.full(shape, -1, dtype=torch.int32, device=q.device)
-        elif out.shape != shape or out.dtype != torch.int32 or not out.is_contiguous() or not out.is_cuda:
-            raise ValueError("out must be a contiguous int32 device tensor [n_seq, q_len, n_kv_heads, n_select]")
-        a = self._args(_capi.PageSelectArgs)
-        a.q, a.pages = q.data_ptr(), out.data_ptr()
-        a.seq_lens, a.q_lens = _lens(seq_lens, B, "seq_lens"), _lens(q_lens, B, "q_lens")
-        a.q_len, a.n_heads, a.n_select, a.n_first, a.n_last = L, H, int(n_select), int(first), int(last)
-        L_ = _capi.lib()
-        n = _bytes(workspace)
-        rc = L_.mugen_attn_page_select(ctypes.byref(a), _ptr(workspace), n, _stream(self.device))
-        if rc == _capi.E_WORKSPACE and workspace is None:
-            n = L_.mugen_attn_page_select_workspace_size(ctypes.byref(a))
-            workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
-            rc = L_.mugen_attn_page_select(ctypes.byref(a), _ptr(workspace), n, _stream(self.device))
-        _capi.check(rc)
+            out = torch.full(shape, -1, dtype=_i32, device=q.device)
+        else:
+            self._like(out, shape, "out", _i32)
+        args = self._store + _SELECT.pack(
+            q.data_ptr(), out.data_ptr(), self._lens(seq_lens, "seq_lens"), self._lens(q_lens, "q_lens"), qs[1], qs[2],
+            n_select, first, last)
+        self._run("page_select", args, workspace)
         return out
 
     # ------------------------------------------------------------- prefill
-
-    def _prefill_args(self, n_tokens: int, n_heads: int, seq: int, start_pos: int, scale: float, out_dtype):
-        a = self._args(_capi.GqaPrefillPagedArgs)
-        a.seq, a.n_tokens, a.start_pos, a.n_heads = int(seq), int(n_tokens), int(start_pos), int(n_heads)
-        a.scale, a.out_dtype = float(scale), _dt(out_dtype)
-        return a
 
     def prefill(self, q: torch.Tensor, seq: int, start_pos: int, *, out: torch.Tensor | None = None,
                 out_dtype: torch.dtype | None = None, scale: float = 0.0,
                 workspace: torch.Tensor | None = None) -> torch.Tensor:
         """Causal attention of a prompt chunk q [n_tokens, n_heads, head_dim] of
         sequence `seq`, already appended at start_pos, over the cache."""
-        _need_cuda(q)
-        if q.dim() != 3 or q.shape[2] != self.head_dim or q.dtype != self.dtype:
+        shape = q.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or q.dtype is not self.dtype:
             raise ValueError("q must be [n_tokens, n_heads, head_dim] in the store's dtype")
+        if q.get_device() != self._index or not q.is_contiguous():
+            raise ValueError("q must be a contiguous tensor on the store's device (no CPU path)")
         if out is None:
-            out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
-        elif out.shape != q.shape or not out.is_contiguous() or not out.is_cuda:
-            raise ValueError("out must be a contiguous device tensor like q")
-        a = self._prefill_args(q.shape[0], q.shape[1], seq, start_pos, scale, out.dtype)
-        a.q, a.out = q.data_ptr(), out.data_ptr()
-        L = _capi.lib()
-        n = _bytes(workspace)
-        rc = L.mugen_attn_gqa_prefill_paged(ctypes.byref(a), _ptr(workspace), n, _stream(self.device))
-        if rc == _capi.E_WORKSPACE and workspace is None:
-            n = L.mugen_attn_gqa_prefill_paged_workspace_size(ctypes.byref(a))
-            workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
-            rc = L.mugen_attn_gqa_prefill_paged(ctypes.byref(a), _ptr(workspace), n, _stream(self.device))
-        _capi.check(rc)
+            out = torch.empty(shape, dtype=out_dtype or q.dtype, device=q.device)
+        else:
+            self._like(out, shape, "out")
+        args = self._store + _PREFILL.pack(q.data_ptr(), out.data_ptr(), seq, shape[0], start_pos, shape[1], scale,
+                                           _dt(out.dtype))
+        self._run("gqa_prefill_paged", args, workspace)
         return out
 
     def prefill_workspace(self, n_tokens: int, n_heads: int, start_pos: int = 0) -> torch.Tensor:
         """The workspace of a prefill call of this shape."""
-        a = self._prefill_args(n_tokens, n_heads, 0, start_pos, 0.0, self.dtype)
-        a.q = a.out = 16  # placeholders
-        need = _capi.lib().mugen_attn_gqa_prefill_paged_workspace_size(ctypes.byref(a))
+        need = _library().gqa_prefill_paged_size(
+            self._store + _PREFILL.pack(16, 16, 0, n_tokens, start_pos, n_heads, 0.0, self._dt16))  # (placeholders)
         return torch.empty(need, dtype=torch.uint8, device=self.device)
 
 
