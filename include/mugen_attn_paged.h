@@ -144,7 +144,7 @@ typedef struct mugen_attn_gqa_decode_paged_args {
     int32_t n_select;      /* entries per list (with pages) */
     int32_t q_len;         /* 1 .. MUGEN_ATTN_PAGED_MAX_Q */
     int32_t n_heads;
-    int32_t num_splits; /* 0: automatic */
+    int32_t num_splits; /* 0: automatic; at most 128 */
     float scale;        /* <= 0: 1 / sqrt(head_dim) */
     int32_t out_dtype;
     const int32_t* seq_lens_host; /* as in mugen_attn_gqa_decode_args */

@@ -74,6 +74,20 @@ struct PagedDecodeParams {
     int* plan;
 };
 
+// most splits of a range
+constexpr int kPagedMaxSplits = 128;
+// A workgroup: WR waves take a tile's 16-row blocks side by side, tile_waves(WR)
+// tiles are under way
+__host__ __device__ constexpr int tile_waves(int WR) { return WR == 1 ? 4 : WR <= 3 ? 2 : 1; }
+// waves that the registers of a SIMD hold: operands of a tile and of the next one
+// (8-bit: half the bytes), O and q
+__host__ __device__ constexpr int paged_waves_per_simd(int D, bool bits8) {
+    return D == 256 ? 1 : D == 128 ? (bits8 ? 3 : 2) : (bits8 ? 4 : 3);
+}
+__host__ __device__ constexpr int paged_groups_per_cu(int D, bool bits8, int WR) {
+    return 4 * paged_waves_per_simd(D, bits8) / (WR * tile_waves(WR));
+}
+
 struct PageSelectParams {
     PagedStore st;
     const uint16_t* q;

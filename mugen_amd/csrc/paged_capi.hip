@@ -203,7 +203,7 @@ int64_t range_len(const mugen_attn_gqa_decode_paged_args* a, int x) {
 }
 
 // most splits of a range: 32, more only in pieces of 512 tokens and up
-constexpr int kCap = 32, kCapLong = 128, kCapTokens = 512, kChunkMin = 64;
+constexpr int kCap = 32, kCapLong = kPagedMaxSplits, kCapTokens = 512, kChunkMin = 64;
 int split_cap(int64_t len) { return (int)std::max<int64_t>(kCap, std::min<int64_t>(kCapLong, len / kCapTokens)); }
 int split_bound(int64_t len) { return (int)std::min<int64_t>(split_cap(len), ceil_div(len, kChunkMin)); }
 
@@ -218,7 +218,7 @@ int64_t decode_items(const mugen_attn_gqa_decode_paged_args* a, int chunk, int64
 size_t decode_bytes(const mugen_attn_gqa_decode_paged_args* a, int splits) {
     if (splits <= 1) return 0;
     const size_t rows = (size_t)a->store.n_seq * a->q_len * a->n_heads;
-    return rows * splits * ((size_t)a->store.head_dim * 4 + 8) + 512;  // alignment, and the planned chunk
+    return 512 + rows * splits * ((size_t)a->store.head_dim * 4 + 8);  // (512: alignment, and the planned chunk)
 }
 
 DecodePlan decode_plan(const mugen_attn_gqa_decode_paged_args* a, bool for_size) {
@@ -228,7 +228,7 @@ DecodePlan decode_plan(const mugen_attn_gqa_decode_paged_args* a, bool for_size)
     r.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 48 && s.head_dim < 256 ? 3 : 4;
     r.nrb = (int)ceil_div(rows, 16 * r.wr);
     const int64_t mult = (int64_t)s.n_kv_heads * r.nrb;
-    r.budget = s.head_dim == 256 || r.wr > 1 ? 256 : 512;
+    r.budget = 256 * paged_groups_per_cu(s.head_dim, s.page_bits == 8, r.wr);
     const int64_t longest = longest_range(a);
     int64_t len = 1;
     for (int x = 0, R = a->seq_lens_host ? ranges_of(a) : 1; x < R; x++) len = std::max(len, range_len(a, x));
@@ -281,8 +281,8 @@ int decode_validate(const mugen_attn_gqa_decode_paged_args* a) {
     if (!aligned16(a->q)) return fail(MUGEN_ATTN_E_INVALID, "%s: q must be 16-byte aligned", who);
     if (a->q_len <= 0 || a->q_len > MUGEN_ATTN_PAGED_MAX_Q)
         return fail(MUGEN_ATTN_E_UNSUPPORTED, "%s: q_len %d (supported: 1 .. %d)", who, a->q_len, MUGEN_ATTN_PAGED_MAX_Q);
-    if (a->num_splits < 0 || a->num_splits > 1024)
-        return fail(MUGEN_ATTN_E_INVALID, "%s: num_splits %d (0 .. 1024)", who, a->num_splits);
+    if (a->num_splits < 0 || a->num_splits > kPagedMaxSplits)
+        return fail(MUGEN_ATTN_E_INVALID, "%s: num_splits %d (0 .. %d)", who, a->num_splits, kPagedMaxSplits);
     if (a->out_dtype != DT_F32 && !is16(a->out_dtype)) return fail(MUGEN_ATTN_E_UNSUPPORTED, "%s: bad out_dtype", who);
     if (a->pages && a->n_select <= 0) return fail(MUGEN_ATTN_E_INVALID, "%s: page lists need n_select > 0", who);
     if (!(a->scale == a->scale) || std::isinf(a->scale)) return fail(MUGEN_ATTN_E_INVALID, "%s: scale is not finite", who);

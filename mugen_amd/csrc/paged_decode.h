@@ -34,9 +34,13 @@
 //    weighted 0: 0 * inf is NaN.  Tiles that reach past the first query's last token
 //    are checked for values that are not finite; where one is met, each token's
 //    rows get their own product with the later rows zeroed;
-//  * the WT waves of a row block merge (m, l, o) through LDS; with one split the result is
-//    stored, otherwise fp32 partials go to the workspace and the combine merges
-//    them.
+//  * the WT waves of a row block merge (m, l, o) through LDS.  A range in one split
+//    stores its result; otherwise fp32 partials go to the workspace and the combine
+//    merges them.  (Merging in the workgroup that counts itself last instead saves
+//    the launch, 3.7 us of host time, but the written-through partials, the count and
+//    the merge follow one another at the end of the longest chain: 5 drafted tokens over
+//    4 x 31k 50 -> 63 us, one sequence of 4096 8.8 -> 11.4, and the workspace would have
+//    to be cleared once.)
 #pragma once
 #include "paged.h"
 
@@ -97,17 +101,10 @@ __device__ __forceinline__ int plan(const PagedDecodeParams& p) {
         [&](int j, int c, float rc) { return max(1, ceil_div_f(units(j), c, rc)); });
 }
 
-// waves that take a tile's row blocks side by side (WR), and tiles under way
-// (WT): 8 waves are what two to a SIMD hold, 4 at head_dim 256, where a wave's
-// operands need a whole SIMD's registers
-__host__ __device__ constexpr int tile_waves(int D, int WR) {
-    return D == 256 ? 4 / WR : WR <= 2 ? 4 : 2;
-}
-
 template <int D, int DT, bool BITS8, int WR, bool LIST>
-__global__ __launch_bounds__(64 * WR * tile_waves(D, WR))
-    __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void paged_decode_kernel(PagedDecodeParams p) {
-    constexpr int WT = tile_waves(D, WR), NW = WR * WT, STEP = 32 * WT;
+__global__ __launch_bounds__(64 * WR * tile_waves(WR))
+    __attribute__((amdgpu_waves_per_eu(paged_waves_per_simd(D, BITS8)))) void paged_decode_kernel(PagedDecodeParams p) {
+    constexpr int WT = tile_waves(WR), NW = WR * WT, STEP = 32 * WT;
     constexpr int KK = D / 32;          // MFMA k-steps of S
     constexpr int KJ = D / 64;          // 16-byte loads of an 8-bit K row per lane
     constexpr int DB = D / 16;          // 16-dim blocks of O^T
@@ -141,7 +138,7 @@ __global__ __launch_bounds__(64 * WR * tile_waves(D, WR))
     const int range = range_of<LIST>(p, j);
     const int t_begin = s * chunk, t_end = min(t_begin + chunk, range);
     if (p.chunk == 0 && blockIdx.x == 0 && threadIdx.x == 0) *p.plan = chunk;  // for the merge
-    if (p.num_splits > 1 && t_begin >= t_end) return;  // nothing to see: the merge skips it
+    const int n_act = min(p.num_splits, max(1, (range + chunk - 1) / chunk));  // splits of this range
     const int G = p.G, wg_row = rb * WR * 16, n_rows = (LIST ? 1 : len.n) * G;
     if (wg_row >= n_rows) return;  // rows of tokens that are not there
     const int wr = w % WR, wt = w / WR, first_row = wg_row + 16 * wr;
@@ -547,35 +544,46 @@ __global__ __launch_bounds__(64 * WR * tile_waves(D, WR))
             f[x] = mw == kNegInf ? 0.f : fast_exp2(mw - M);
             L += f[x] * l_lds[at(x)];
         }
-        const float c = p.num_splits == 1 ? (L > 0.f ? 1.f / L : L == L ? 0.f : L) : 1.f;
+        const float c = n_act == 1 ? (L > 0.f ? 1.f / L : L == L ? 0.f : L) : 1.f;
 #pragma unroll
         for (int x = 0; x < WT; x++) f_lds[at(x)] = f[x] * c;
         ml_out[2 * h] = M;
         ml_out[2 * h + 1] = L;
     }
     __syncthreads();
-    for (int idx = threadIdx.x; idx < WR * 16 * D; idx += 64 * NW) {
-        const int h = idx / D, d = idx - h * D, r2 = wg_row + h;
-        if (r2 >= n_rows) break;
-        const int i = LIST ? i0 : r2 / G, hh = LIST ? r2 : r2 - i * G;
-        float O = 0.f;
+    const int rows_here = min(WR * 16, n_rows - wg_row);
+    // row r of the workgroup in q and out
+    auto out_row = [&](int r2) {
+        const int i = LIST ? i0 : (wg_row + r2) / G;
+        return ((int64_t)b * p.q_len + i) * p.H + kvh * G + (LIST ? r2 : wg_row + r2 - i * G);
+    };
+    auto store4 = [&](int64_t orow, int d, f32x4_t v) {
+        if (p.out_dt == DT_F32) {
+            *reinterpret_cast<f32x4_t*>(static_cast<float*>(p.out) + orow * D + d) = v;
+        } else {
+            const u32x2_t x = p.out_dt == DT_F16 ? u32x2_t{pack2<DT_F16>(v[0], v[1]), pack2<DT_F16>(v[2], v[3])}
+                                                 : u32x2_t{pack2<DT_BF16>(v[0], v[1]), pack2<DT_BF16>(v[2], v[3])};
+            *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p.out) + orow * D + d) = x;
+        }
+    };
+    for (int idx = threadIdx.x; idx < rows_here * (D / 4); idx += 64 * NW) {
+        const int h = idx / (D / 4), d = 4 * (idx % (D / 4));
+        f32x4_t O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < WT; x++) {
             const int at = (x * WR + (h >> 4)) * 16 + (h & 15);
             const float f = f_lds[at];
-            O += f == 0.f ? 0.f : f * o_lds[at * OROW + d];
+            if (f != 0.f) O += f * *reinterpret_cast<const f32x4_t*>(&o_lds[at * OROW + d]);
         }
-        const int64_t orow = ((int64_t)b * p.q_len + i) * p.H + kvh * G + hh;
-        if (p.num_splits == 1) {
-            if (p.out_dt == DT_F32) store_out<DT_F32>(p.out, orow * D + d, O);
-            else if (p.out_dt == DT_F16) store_out<DT_F16>(p.out, orow * D + d, O);
-            else store_out<DT_BF16>(p.out, orow * D + d, O);
+        const int64_t orow = out_row(h);
+        if (n_act == 1) {
+            store4(orow, d, O);
         } else {
             const int64_t slot = orow * p.num_splits + s;
-            p.ws_o[slot * D + d] = O;
+            store_wt(reinterpret_cast<u32x4_t*>(p.ws_o + slot * D + d), __builtin_bit_cast(u32x4_t, O));
             if (d == 0) {
-                p.ws_ml[slot * 2] = ml_out[2 * h];
-                p.ws_ml[slot * 2 + 1] = ml_out[2 * h + 1];
+                store_wt(p.ws_ml + slot * 2, ml_out[2 * h]);
+                store_wt(p.ws_ml + slot * 2 + 1, ml_out[2 * h + 1]);
             }
         }
     }
@@ -586,7 +594,7 @@ hipError_t launch_rows(const PagedDecodeParams& p, int nwg, int wr, hipStream_t 
     auto go = [&](auto r, auto list) {
         constexpr int WR = decltype(r)::value;
         return launch_k(t, "gqa_decode_paged", paged_decode_kernel<D, DT, BITS8, WR, decltype(list)::value>, dim3(nwg),
-                        dim3(64 * WR * tile_waves(D, WR)), st, p);
+                        dim3(64 * WR * tile_waves(WR)), st, p);
     };
     if (p.sel) return go(std::integral_constant<int, 1>{}, std::true_type{});
     if (wr == 1) return go(std::integral_constant<int, 1>{}, std::false_type{});

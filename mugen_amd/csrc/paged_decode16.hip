@@ -17,6 +17,7 @@ __global__ __launch_bounds__(64) void paged_combine_kernel(PagedDecodeParams p) 
     const int chunk = p.chunk ? p.chunk : *p.plan;
     const int range = paged::range_of<LIST>(p, LIST ? (int)blockIdx.y : b);
     const int nact = min(p.num_splits, (range + chunk - 1) / chunk);
+    if (nact <= 1) return;  // one split: the result is there
     const int64_t row = (int64_t)blockIdx.y * p.H + h;
     const float* ml = p.ws_ml + row * p.num_splits * 2;
     const float* os = p.ws_o + row * p.num_splits * D + d;
