@@ -44,7 +44,7 @@ extern "C" {
  * the maximum of each dim over a whole page's keys, for
  * mugen_attn_page_select.
  *
- * page_table entries past a sequence's pages are not read.  An entry outside
+ * page_table entries past a sequence's pages may be anything.  An entry outside
  * [0, n_pages) is a page that is not there: attention leaves its tokens out,
  * an append drops them.  No two sequences may append to one page (full pages
  * may be shared).

@@ -13,9 +13,10 @@
 // (sequence, touched page, kv head, tensor) forms a page that these tokens
 // fill from the rows that were there (ring or page) and the new ones, all in
 // registers: magnitude, exponent, codes in one pass.  It rotates the new rows
-// itself, so it need not wait for the row threads; the ring slots it reads are not
-// written by the same launch (the host sends the rows in a launch of their own
-// where the new tokens could wrap around to them).
+// itself, so it need not wait for the row threads.  The ring slots of the open page's
+// held rows, which the page job reads, are its own to write too: where a long prompt's
+// newest tokens wrap around to them, the row threads leave those slots alone and the job
+// writes them once it holds the old rows.
 // The least e with amax <= 448 * 2^e: amax = m 2^x, 0.5 <= m < 1, is
 // m * 2^(x-9) * 512, so e = x - 9 where m <= 448/512, else x - 8: no division.
 #include "paged.h"
@@ -27,7 +28,8 @@ namespace {
 struct Turn8 {
     float c[8], s[8];
 };
-__device__ __forceinline__ Turn8 turn8(const RopeTurns& t, int u, int pos) {
+template <int N>
+__device__ __forceinline__ Turn8 turn8(const RopeTurns<N>& t, int u, int pos) {
     Turn8 r;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -62,8 +64,15 @@ __device__ __forceinline__ void append_lens(const PagedAppendParams& p, int b, i
     T_out = n < p.st.max_T - T ? T + n : p.st.max_T;
 }
 
+// 8-bit: new token `pos` goes to a ring slot that holds a row of the open page while
+// a page job fills that page
+__device__ __forceinline__ bool page_jobs_slot(const PagedAppendParams& p, int T, int T_out, int pos) {
+    const int P = 1 << p.st.p_shift, open = T & -P;  // first token of the open page
+    return T_out >= open + P && ((pos - open) & (p.st.ring - 1)) < T - open;
+}
+
 template <int D, int DT, bool BITS8>
-__device__ __forceinline__ void append_rows(const PagedAppendParams& p, uint32_t thread) {
+__device__ __forceinline__ void append_rows(const PagedAppendParams& p, const RopeTurns<D / 2>& turns, uint32_t thread) {
     constexpr uint32_t U = D / 16;
     const int hpt = p.heads_per_thread, heads = p.H + 2 * p.st.Hk;
     const uint32_t groups = (uint32_t)(heads + hpt - 1) / (uint32_t)hpt;
@@ -83,7 +92,7 @@ __device__ __forceinline__ void append_rows(const PagedAppendParams& p, uint32_t
     const bool rot = 16 * u < p.rope_dim;
     const int h_end = min((hg + 1) * hpt, heads);
     Turn8 turn{};
-    if (rot && hg * hpt < p.H + p.st.Hk) turn = turn8(p.turns, u, pos);  // (V heads come last)
+    if (rot && hg * hpt < p.H + p.st.Hk) turn = turn8(turns, u, pos);  // (V heads come last)
     for (int h = hg * hpt; h < h_end; h++) {
         const uint16_t* src;
         uint16_t* dst;
@@ -96,6 +105,7 @@ __device__ __forceinline__ void append_rows(const PagedAppendParams& p, uint32_t
             src = (is_v ? p.v_new + id * p.v_stride : p.k_new + id * p.k_stride) + (int64_t)kvh * D;
             if constexpr (BITS8) {
                 if (pos < T_out - p.st.ring) continue;  // pushed out of the ring by this call's own tokens
+                if (page_jobs_slot(p, T, T_out, pos)) continue;
                 dst = (is_v ? p.st.tail_v : p.st.tail_k) + b * p.st.tail_stride +
                       ((int64_t)(pos & (p.st.ring - 1)) * p.st.Hk + kvh) * D;
             } else {
@@ -118,7 +128,7 @@ __device__ __forceinline__ float nan_max(float a, float b) { return (b > a || b 
 
 // the page that job `id` is about, where this call fills it
 template <int D, int P, int DT, bool BITS8>
-__device__ __forceinline__ void append_page(const PagedAppendParams& p, int id, char* lds) {
+__device__ __forceinline__ void append_page(const PagedAppendParams& p, const RopeTurns<D / 2>& turns, int id, char* lds) {
     constexpr int U = D / 16, UNITS = P * U, UPT = (UNITS + 255) / 256;
     // job = ((b * pages + c) * tensors + tensor) * Hk + kvh
     const int Hk = p.st.Hk;
@@ -135,7 +145,7 @@ __device__ __forceinline__ void append_page(const PagedAppendParams& p, int id, 
     const int page = T / P + c;
     if (page >= T_out / P) return;  // not filled by this call
     const int phys = checked_page(p.st.table[b * p.st.table_stride + page], p.st.n_pages);
-    if (phys < 0) return;
+    if (phys < 0 && !(BITS8 && c == 0)) return;  // (its ring slots are still this job's)
     const int64_t ph = (int64_t)phys * Hk + kvh;
     const bool ranged = !is_v && p.st.k_range;
     u32x4_t xa[UPT], xb[UPT];
@@ -153,7 +163,7 @@ __device__ __forceinline__ void append_page(const PagedAppendParams& p, int id, 
             const uint16_t* src = (is_v ? p.v_new + row * p.v_stride : p.k_new + row * p.k_stride) + (int64_t)kvh * D;
             xa[i] = load16(src + d0);
             xb[i] = load16(src + d1);
-            if (!is_v && 16 * u < p.rope_dim) rotate8<DT>(turn8(p.turns, u, t), xa[i], xb[i]);
+            if (!is_v && 16 * u < p.rope_dim) rotate8<DT>(turn8(turns, u, t), xa[i], xb[i]);
         } else {
             const uint16_t* src;
             if constexpr (BITS8)
@@ -178,9 +188,29 @@ __device__ __forceinline__ void append_page(const PagedAppendParams& p, int id, 
         float* red = reinterpret_cast<float*>(lds);
         amax = wave_max(amax);
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
-        __syncthreads();
+        __syncthreads();  // (and every old row of the page is in registers)
         amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         __syncthreads();
+        if (c == 0) {
+            // the newest tokens whose slots those rows had
+            const int held = T - page * P;
+            for (int unit = threadIdx.x; unit < held * U; unit += 256) {
+                const int r = unit / U, u = unit % U, slot = (page * P + r) & (p.st.ring - 1);
+                // the last token before T_out at this slot
+                const int t = T_out - 1 - ((T_out - 1 - slot) & (p.st.ring - 1));
+                if (t < T) continue;
+                int d0, d1;
+                unit_dims(u, p.rope_dim, d0, d1);
+                const int64_t row = (int64_t)b * p.n_new + (t - T);
+                const uint16_t* src = (is_v ? p.v_new + row * p.v_stride : p.k_new + row * p.k_stride) + (int64_t)kvh * D;
+                u32x4_t x = load16(src + d0), y = load16(src + d1);
+                if (!is_v && 16 * u < p.rope_dim) rotate8<DT>(turn8(turns, u, t), x, y);
+                uint16_t* dst = (is_v ? p.st.tail_v : p.st.tail_k) + b * p.st.tail_stride + ((int64_t)slot * Hk + kvh) * D;
+                *reinterpret_cast<u32x4_t*>(dst + d0) = x;
+                *reinterpret_cast<u32x4_t*>(dst + d1) = y;
+            }
+        }
+        if (phys < 0) return;
         byte = 1;
         if (amax > 0.f) {
             int x;
@@ -284,16 +314,16 @@ __device__ __forceinline__ void append_page(const PagedAppendParams& p, int id, 
 constexpr int kPageLds = 256 * 17 * 4;  // the ranges' partials; at least a page's V codes (32 KiB) where those are wider
 
 template <int D, int DT, bool BITS8>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) {
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p, RopeTurns<D / 2> turns) {
     if ((int)blockIdx.x < p.row_blocks) {
-        append_rows<D, DT, BITS8>(p, blockIdx.x * 256u + threadIdx.x);
+        append_rows<D, DT, BITS8>(p, turns, blockIdx.x * 256u + threadIdx.x);
         return;
     }
     __shared__ __attribute__((aligned(16))) char lds[kPageLds > 128 * D ? kPageLds : 128 * D];
     const int id = (int)blockIdx.x - p.row_blocks;
-    if (p.st.p_shift == 5) append_page<D, 32, DT, BITS8>(p, id, lds);
-    else if (p.st.p_shift == 6) append_page<D, 64, DT, BITS8>(p, id, lds);
-    else append_page<D, 128, DT, BITS8>(p, id, lds);
+    if (p.st.p_shift == 5) append_page<D, 32, DT, BITS8>(p, turns, id, lds);
+    else if (p.st.p_shift == 6) append_page<D, 64, DT, BITS8>(p, turns, id, lds);
+    else append_page<D, 128, DT, BITS8>(p, turns, id, lds);
 }
 
 // 32 tokens of one kv head: pages (or ring) -> [T][Hk * D] rows
@@ -373,28 +403,20 @@ hipError_t by_shape(int D, int dt, bool bits8, F f) {
     return by_dt(std::integral_constant<int, 64>{});
 }
 
-hipError_t launch_append(PagedAppendParams p, int D, int dt, bool bits8, bool rows, bool pages, hipStream_t st,
-                         KernelTimer* t) {
-    const int heads = p.H + 2 * p.st.Hk, groups = (heads + p.heads_per_thread - 1) / p.heads_per_thread;
-    const int64_t threads = (int64_t)p.n_seq * p.n_new * groups * (D / 16);
-    p.row_blocks = rows ? (int)((threads + 255) / 256) : 0;
-    const int jobs = pages ? p.n_seq * p.pages * p.st.Hk * (bits8 ? 2 : 1) : 0;
-    if (p.row_blocks + jobs == 0) return hipSuccess;
-    return by_shape(D, dt, bits8, [&](auto d, auto e, auto b8) {
-        return launch_k(t, "kv_paged_append", paged_append_kernel<decltype(d)::value, decltype(e)::value, decltype(b8)::value>,
-                        dim3(p.row_blocks + jobs), dim3(256), st, p);
-    });
-}
-
 }  // namespace
 
-hipError_t launch_paged_append(const PagedAppendParams& p, int D, int dt, bool bits8, hipStream_t st, KernelTimer* t) {
-    const bool pages = bits8 || p.st.k_range;
-    // one launch where the new tokens' ring slots cannot be those of the rows
-    // that a filled page takes from the ring
-    if (!bits8 || p.n_new + (1 << p.st.p_shift) <= p.st.ring) return launch_append(p, D, dt, bits8, true, pages, st, t);
-    const hipError_t e = launch_append(p, D, dt, bits8, false, true, st, t);
-    return e != hipSuccess ? e : launch_append(p, D, dt, bits8, true, false, st, t);
+hipError_t launch_paged_append(PagedAppendParams p, const RopeTurns<128>& turns, int D, int dt, bool bits8, hipStream_t st, KernelTimer* t) {
+    const int heads = p.H + 2 * p.st.Hk, groups = (heads + p.heads_per_thread - 1) / p.heads_per_thread;
+    const int64_t threads = (int64_t)p.n_seq * p.n_new * groups * (D / 16);
+    p.row_blocks = (int)((threads + 255) / 256);
+    const int jobs = bits8 || p.st.k_range ? p.n_seq * p.pages * p.st.Hk * (bits8 ? 2 : 1) : 0;
+    return by_shape(D, dt, bits8, [&](auto d, auto e, auto b8) {
+        constexpr int DD = decltype(d)::value;
+        RopeTurns<DD / 2> f;
+        for (int i = 0; i < DD / 2; i++) f.f[i] = turns.f[i];
+        return launch_k(t, "kv_paged_append", paged_append_kernel<DD, decltype(e)::value, decltype(b8)::value>,
+                        dim3(p.row_blocks + jobs), dim3(256), st, p, f);
+    });
 }
 
 hipError_t launch_paged_gather(const PagedGatherParams& p, int D, int dt, bool bits8, hipStream_t st, KernelTimer* t) {

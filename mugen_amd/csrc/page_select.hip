@@ -48,48 +48,63 @@ __device__ __forceinline__ int pages_seen(const PageSelectParams& p, int T, int 
     return (max(T - n + i + 1, 0) + (1 << p.st.p_shift) - 1) >> p.st.p_shift;
 }
 
-constexpr int kScorePages = 64;  // pages of a score workgroup: 16 a step
-constexpr int kScoreQueries = 8;  // queries whose Q-, Q+ are held at a time
+// pages of a score workgroup, 16 a step: all their ranges are in flight at once, and
+// the group's queries are summed meanwhile
+template <int D>
+constexpr int score_pages() { return D == 64 ? 128 : D == 128 ? 64 : 32; }
+constexpr int kScoreQueries = 4;  // queries whose Q-, Q+ are held at a time
 
 template <int D, int DT>
 __global__ __launch_bounds__(256) void page_score_kernel(PageSelectParams p) {
     constexpr int C = 2 * D / 128;  // 16-byte loads of a lane per page
-    constexpr int STEPS = kScorePages / 16;
+    constexpr int PAGES = score_pages<D>(), STEPS = PAGES / 16;
     __shared__ double Q[kScoreQueries][2 * D];
-    const int kvh = blockIdx.y, b = blockIdx.z, page0 = blockIdx.x * kScorePages;
+    const int kvh = blockIdx.y, b = blockIdx.z, page0 = blockIdx.x * PAGES;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15;
+    // this wave's pages: page0 + 16 * step + 4 * wave + lane / 16.  Their table entries
+    // do not wait for the length (max_pages bounds them)
+    int phys[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; s++)
+        phys[s] = p.st.table[b * p.st.table_stride + min(page0 + 16 * s + 4 * wave + (lane >> 4), p.max_pages - 1)];
     const int T = select_len(p, b), n = select_new(p, b);
     if (n == 0) return;
     // candidates of the last query, the one that sees most
     const int end = pages_seen(p, T, n, n - 1) - p.n_last;
-    if (page0 >= end || page0 + kScorePages <= p.n_first || end + p.n_last <= p.n_select) return;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15;
-    // this wave's pages: page0 + 16 * step + 4 * wave + lane / 16
+    if (page0 >= end || page0 + PAGES <= p.n_first || end + p.n_last <= p.n_select) return;
     u32x4_t raw[STEPS][C];
-    bool there[STEPS];
 #pragma unroll
     for (int s = 0; s < STEPS; s++) {
-        const int page = page0 + 16 * s + 4 * wave + (lane >> 4);
-        int phys = -1;
-        if (page < end) phys = checked_page(p.st.table[b * p.st.table_stride + page], p.st.n_pages);
-        there[s] = phys >= 0;
-        const uint16_t* src = p.st.k_range + ((int64_t)max(phys, 0) * p.st.Hk + kvh) * 2 * D;
+        // (entries past the pages that are seen may be anything)
+        if (page0 + 16 * s + 4 * wave + (lane >> 4) >= end) phys[s] = -1;
+        phys[s] = checked_page(phys[s], p.st.n_pages);
+        const uint16_t* src = p.st.k_range + ((int64_t)max(phys[s], 0) * p.st.Hk + kvh) * 2 * D;
 #pragma unroll
         for (int c = 0; c < C; c++) raw[s][c] = load16(src + 8 * (16 * c + l16));
     }
     for (int i0 = 0; i0 < n; i0 += kScoreQueries) {
         const int ni = min(kScoreQueries, n - i0);
-        __syncthreads();
-        for (int x = threadIdx.x; x < ni * D; x += 256) {
-            const int i = x / D, d = x - i * D;
+        if (i0) __syncthreads();
+        for (int x = threadIdx.x; x < ni * (D / 2); x += 256) {  // two dims a thread
+            const int i = x / (D / 2), d = 2 * (x - i * (D / 2));
             const uint16_t* q = p.q + (((int64_t)b * p.q_len + i0 + i) * p.H + (int64_t)kvh * p.G) * D + d;
-            double neg = 0.0, pos = 0.0;
-            for (int h = 0; h < p.G; h++) {
-                const double v = (double)to_f32<DT>(q[h * D]);
-                if (v < 0.0) neg += v;
-                else pos += v;  // (a NaN too)
+            uint32_t w[16];
+#pragma unroll
+            for (int h = 0; h < 16; h++) w[h] = *reinterpret_cast<const uint32_t*>(q + min(h, p.G - 1) * D);
+            double neg0 = 0.0, pos0 = 0.0, neg1 = 0.0, pos1 = 0.0;
+#pragma unroll
+            for (int h = 0; h < 16; h++) {
+                if (h >= p.G) break;
+                const double v0 = (double)lo_f32<DT>(w[h]), v1 = (double)hi_f32<DT>(w[h]);
+                neg0 += v0 < 0.0 ? v0 : 0.0;
+                pos0 += v0 < 0.0 ? 0.0 : v0;  // (a NaN too)
+                neg1 += v1 < 0.0 ? v1 : 0.0;
+                pos1 += v1 < 0.0 ? 0.0 : v1;
             }
-            Q[i][d] = neg;
-            Q[i][D + d] = pos;
+            Q[i][d] = neg0;
+            Q[i][d + 1] = neg1;
+            Q[i][D + d] = pos0;
+            Q[i][D + d + 1] = pos1;
         }
         __syncthreads();
 #pragma unroll
@@ -104,15 +119,15 @@ __global__ __launch_bounds__(256) void page_score_kernel(PageSelectParams p) {
                 }
             const int page = page0 + 16 * s + 4 * wave + (lane >> 4);
             for (int i = 0; i < ni; i++) {
-                double sum = 0.0;
+                double part[2] = {0.0, 0.0};  // (two chains: an fma takes 8 cycles to come back)
 #pragma unroll
                 for (int c = 0; c < C; c++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) sum = fma(Q[i][8 * (16 * c + l16) + e], x[8 * c + e], sum);
-                sum = row_sum16(sum) + 0.0;  // (-0 counts as 0)
+                    for (int e = 0; e < 8; e++) part[e & 1] = fma(Q[i][8 * (16 * c + l16) + e], x[8 * c + e], part[e & 1]);
+                double sum = row_sum16(part[0] + part[1]) + 0.0;  // (-0 counts as 0)
                 uint64_t key = __builtin_bit_cast(uint64_t, sum);
                 key = sum != sum ? ~0ull : (key >> 63) ? ~key : key | (1ull << 63);
-                if (!there[s]) key = 0;
+                if (phys[s] < 0) key = 0;
                 if (l16 == 0 && page < end)
                     p.keys[(((int64_t)b * p.q_len + i0 + i) * p.st.Hk + kvh) * p.max_pages + page] = key;
             }
@@ -257,7 +272,7 @@ __global__ __launch_bounds__(64 * WAVES) void page_select_kernel(PageSelectParam
 
 template <int D>
 hipError_t launch_score_d(const PageSelectParams& p, int dt, hipStream_t st, KernelTimer* t) {
-    const dim3 grid((p.max_pages + kScorePages - 1) / kScorePages, p.st.Hk, p.B);
+    const dim3 grid((p.max_pages + score_pages<D>() - 1) / score_pages<D>(), p.st.Hk, p.B);
     if (dt == DT_F16) return launch_k(t, "page_score", page_score_kernel<D, DT_F16>, grid, dim3(256), st, p);
     return launch_k(t, "page_score", page_score_kernel<D, DT_BF16>, grid, dim3(256), st, p);
 }

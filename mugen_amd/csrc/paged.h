@@ -25,9 +25,11 @@ struct PagedStore {
     int max_T;
 };
 
-// turns per position of each rotated pair: frequency / (2 pi), in 64 bits
+// turns per position of each rotated pair: frequency / (2 pi), in 64 bits (passed
+// by value: head_dim / 2 of them)
+template <int N>
 struct RopeTurns {
-    double f[128];
+    double f[N];
 };
 
 struct PagedAppendParams {
@@ -47,7 +49,6 @@ struct PagedAppendParams {
     int heads_per_thread;
     int row_blocks;   // workgroups of row work, ahead of the page jobs
     int pages;        // page jobs per (sequence, kv head, tensor): the pages n_new tokens can touch
-    RopeTurns turns;
 };
 
 struct PagedDecodeParams {
@@ -76,16 +77,21 @@ struct PagedDecodeParams {
 
 // most splits of a range
 constexpr int kPagedMaxSplits = 128;
-// A workgroup: WR waves take a tile's 16-row blocks side by side, tile_waves(WR)
-// tiles are under way
-__host__ __device__ constexpr int tile_waves(int WR) { return WR == 1 ? 4 : WR <= 3 ? 2 : 1; }
 // waves that the registers of a SIMD hold: operands of a tile and of the next one
 // (8-bit: half the bytes), O and q
 __host__ __device__ constexpr int paged_waves_per_simd(int D, bool bits8) {
     return D == 256 ? 1 : D == 128 ? (bits8 ? 3 : 2) : (bits8 ? 4 : 3);
 }
+// A workgroup: WR waves take a tile's 16-row blocks side by side, paged_tiles tiles
+// are under way.  4 waves in all, one to a SIMD, or 12 (three row blocks), which
+// fill a CU that holds 3 to a SIMD (two workgroups of 6 do not fit beside each other:
+// 2, 2, 1, 1 waves each; 5 drafted tokens of 28 / 4 heads over 4 x 31k 47 -> 35 us)
+__host__ __device__ constexpr int paged_tiles(int D, bool bits8, int WR) {
+    return WR == 1 ? 4 : WR == 2 ? 2 : WR == 4 ? 1 : paged_waves_per_simd(D, bits8) >= 3 ? 4 : 2;
+}
 __host__ __device__ constexpr int paged_groups_per_cu(int D, bool bits8, int WR) {
-    return 4 * paged_waves_per_simd(D, bits8) / (WR * tile_waves(WR));
+    const int waves = WR * paged_tiles(D, bits8, WR), most = 4 * paged_waves_per_simd(D, bits8);
+    return waves > 4 ? 1 : most / 4;
 }
 
 struct PageSelectParams {
@@ -108,7 +114,7 @@ struct PagedGatherParams {
     int T;
 };
 
-hipError_t launch_paged_append(const PagedAppendParams& p, int D, int dt, bool bits8, hipStream_t st, KernelTimer* t);
+hipError_t launch_paged_append(PagedAppendParams p, const RopeTurns<128>& turns, int D, int dt, bool bits8, hipStream_t st, KernelTimer* t);
 hipError_t launch_paged_gather(const PagedGatherParams& p, int D, int dt, bool bits8, hipStream_t st, KernelTimer* t);
 // wr: 16-row blocks of one workgroup (1 .. 4; 1, 2 or 4 at head_dim 256)
 hipError_t launch_paged_decode16(const PagedDecodeParams& p, int nwg, int D, int dt, int wr, hipStream_t st,

@@ -87,8 +87,8 @@ float* align256(void* p) { return reinterpret_cast<float*>((reinterpret_cast<uin
 // factor > 1 with the YaRN correction of yarn_rope_freq (transformer.cpp:41-70;
 // beta_fast 32, beta_slow 1), in 64 bits (the powers by repeated products in extended
 // precision: a pow() a pair took 3 us of a call)
-RopeTurns rope_turns(const mugen_attn_rope_params& r, int rope_dim) {
-    RopeTurns out{};
+RopeTurns<128> rope_turns(const mugen_attn_rope_params& r, int rope_dim) {
+    RopeTurns<128> out{};
     const double two_pi = 6.283185307179586476925286766559;
     const double theta = r.theta, dim = rope_dim;
     const bool yarn = r.factor > 1.f;
@@ -158,7 +158,8 @@ extern "C" int mugen_attn_kv_paged_append(const mugen_attn_kv_paged_append_args*
     p.n_new = a->n_new;
     p.H = a->q ? a->n_heads : 0;
     p.rope_dim = a->rope_dim;
-    if (a->rope_dim) p.turns = rope_turns(r, a->rope_dim);
+    RopeTurns<128> turns{};
+    if (a->rope_dim) turns = rope_turns(r, a->rope_dim);
     const int heads = p.H + 2 * s.n_kv_heads;
     const int64_t tokens = (int64_t)s.n_seq * a->n_new;
     // one head a thread where the tokens are few (latency), up to 8 where their
@@ -168,7 +169,7 @@ extern "C" int mugen_attn_kv_paged_append(const mugen_attn_kv_paged_append_args*
     const int64_t jobs = (int64_t)s.n_seq * p.pages * s.n_kv_heads * 2;
     if (tokens * heads * (s.head_dim / 16) > INT32_MAX || jobs > INT32_MAX / 2)
         return fail(MUGEN_ATTN_E_UNSUPPORTED, "%s: too many tokens in one call", who);
-    return hip_status(launch_paged_append(p, s.head_dim, s.dtype, s.page_bits == 8, static_cast<hipStream_t>(stream),
+    return hip_status(launch_paged_append(p, turns, s.head_dim, s.dtype, s.page_bits == 8, static_cast<hipStream_t>(stream),
                                           active_timer()),
                       "kv_paged_append launch");
 }

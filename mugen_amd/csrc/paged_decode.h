@@ -102,9 +102,9 @@ __device__ __forceinline__ int plan(const PagedDecodeParams& p) {
 }
 
 template <int D, int DT, bool BITS8, int WR, bool LIST>
-__global__ __launch_bounds__(64 * WR * tile_waves(WR))
+__global__ __launch_bounds__(64 * WR * paged_tiles(D, BITS8, WR))
     __attribute__((amdgpu_waves_per_eu(paged_waves_per_simd(D, BITS8)))) void paged_decode_kernel(PagedDecodeParams p) {
-    constexpr int WT = tile_waves(WR), NW = WR * WT, STEP = 32 * WT;
+    constexpr int WT = paged_tiles(D, BITS8, WR), NW = WR * WT, STEP = 32 * WT;
     constexpr int KK = D / 32;          // MFMA k-steps of S
     constexpr int KJ = D / 64;          // 16-byte loads of an 8-bit K row per lane
     constexpr int DB = D / 16;          // 16-dim blocks of O^T
@@ -594,7 +594,7 @@ hipError_t launch_rows(const PagedDecodeParams& p, int nwg, int wr, hipStream_t 
     auto go = [&](auto r, auto list) {
         constexpr int WR = decltype(r)::value;
         return launch_k(t, "gqa_decode_paged", paged_decode_kernel<D, DT, BITS8, WR, decltype(list)::value>, dim3(nwg),
-                        dim3(64 * WR * tile_waves(WR)), st, p);
+                        dim3(64 * WR * paged_tiles(D, BITS8, WR)), st, p);
     };
     if (p.sel) return go(std::integral_constant<int, 1>{}, std::true_type{});
     if (wr == 1) return go(std::integral_constant<int, 1>{}, std::false_type{});
