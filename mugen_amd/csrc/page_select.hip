@@ -11,11 +11,14 @@
 // a wave instruction; every query of a sequence is scored from one read.
 // Bound: HBM (4 * head_dim bytes a page and kv head).
 //
-// Choice.  Scores become 64-bit integers of the same order, held in registers.  A
-// radix select finds the border: 8 bits a pass from the highest bit in which any two
-// candidates differ, ended as soon as a digit's bin is taken whole, so that a few
-// passes do for scores that are spread.  Equal keys at the border are taken from
-// the lowest page on; two ballots and one scan then place the ascending list.
+// Choice.  Scores become 64-bit integers of the same order, held in registers.  One
+// histogram over 1024 equal bins between the least and the largest score finds the bin
+// of the border; the few keys in it are ranked by one wave.  Where more than 64
+// share the bin (equal or very uneven scores), a radix select takes over: 8 bits a
+// pass from the highest bit in which any two candidates differ, then, among equal
+// keys, over the page number (the lowest pages win).  Either way the choice is a
+// border (key, page), and a ballot with one scan places the ascending list.
+// Bound: latency, a chain of 8 barriers (radix passes alone: 20; 2048 pages 7.7 us).
 #include "paged.h"
 
 namespace mugen_attn {
@@ -135,13 +138,38 @@ __global__ __launch_bounds__(256) void page_score_kernel(PageSelectParams p) {
     }
 }
 
+// minimum (MAX: maximum) over the wave, in every lane
+template <bool MAX>
+__device__ __forceinline__ float wave_least(float v) { return MAX ? wave_max(v) : -wave_max(-v); }
+
+// the bin, counted from the top one, that holds the need-th key: hist[n_bins],
+// n_bins a multiple of 64; leaves (bin, keys wanted in it, keys in it) in `pick`
+__device__ __forceinline__ void find_bin(const uint32_t* hist, int n_bins, int need, int lane, int* pick) {
+    const int per = n_bins / 64, top = n_bins - 1 - per * lane;
+    uint32_t sum = 0;
+    for (int e = 0; e < per; e++) sum += hist[top - e];
+    const int incl = wave_scan_i32((int)sum);
+    if (lane == __builtin_ctzll(__ballot(incl >= need))) {
+        int above = incl - (int)sum, e = 0;
+        while (e < per - 1 && above + (int)hist[top - e] < need) above += (int)hist[top - e++];
+        pick[0] = top - e;
+        pick[1] = need - above;
+        pick[2] = (int)hist[top - e];
+    }
+}
+
 template <int WAVES, int KPT>
 __global__ __launch_bounds__(64 * WAVES) void page_select_kernel(PageSelectParams p) {
-    constexpr int NT = 64 * WAVES;
-    __shared__ uint32_t hist[256];
+    constexpr int NT = 64 * WAVES, BINS = 1024;
+    __shared__ uint32_t hist[BINS];
     __shared__ uint32_t counts[KPT * WAVES];
-    __shared__ uint64_t red[2 * WAVES];
-    __shared__ int pick[2];
+    __shared__ float red[2 * WAVES];
+    __shared__ uint64_t list_key[64];
+    __shared__ int list_page[64];
+    __shared__ uint32_t list_n;
+    __shared__ int pick[3];
+    __shared__ uint64_t border_key;
+    __shared__ int border_page;
     const int kvh = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int T = select_len(p, b), n = select_new(p, b);
@@ -156,118 +184,169 @@ __global__ __launch_bounds__(64 * WAVES) void page_select_kernel(PageSelectParam
     int need = p.n_select - p.n_first - p.n_last;
     const uint64_t* keys = p.keys + (((int64_t)b * p.q_len + i) * p.st.Hk + kvh) * p.max_pages;
     uint64_t key[KPT];
-    uint64_t all = ~0ull, any = 0;  // bits set in every / in some candidate
+    float val[KPT];  // the score in fp32: of the same order, but for equal roundings
+    float lo = -kNegInf, hi = kNegInf;
+    auto cand = [&](int m) { return m * NT + tid >= first && m * NT + tid < end; };
 #pragma unroll
     for (int m = 0; m < KPT; m++) {
-        const int x = m * NT + tid;
-        key[m] = 0;
-        if (x >= first && x < end) {
-            key[m] = keys[x];
-            all &= key[m];
-            any |= key[m];
+        key[m] = cand(m) ? keys[m * NT + tid] : 0;
+        const uint64_t bits = (key[m] >> 63) ? key[m] & ~(1ull << 63) : ~key[m];
+        val[m] = key[m] == ~0ull ? -kNegInf : key[m] == 0 ? kNegInf : (float)__builtin_bit_cast(double, bits);
+        if (cand(m) && fabsf(val[m]) < -kNegInf) {
+            lo = fminf(lo, val[m]);
+            hi = fmaxf(hi, val[m]);
         }
     }
-    for (int d = 32; d; d >>= 1) {
-        all &= __shfl_xor(all, d, 64);
-        any |= __shfl_xor(any, d, 64);
-    }
+    for (int x = tid; x < BINS; x += NT) hist[x] = 0;
+    if (tid == 0) list_n = 0;
+    lo = wave_least<false>(lo);
+    hi = wave_least<true>(hi);
     if (lane == 0) {
-        red[2 * w] = all;
-        red[2 * w + 1] = any;
+        red[2 * w] = lo;
+        red[2 * w + 1] = hi;
     }
     __syncthreads();
-    all = ~0ull, any = 0;
 #pragma unroll
     for (int x = 0; x < WAVES; x++) {
-        all &= red[2 * x];
-        any |= red[2 * x + 1];
+        lo = fminf(lo, red[2 * x]);
+        hi = fmaxf(hi, red[2 * x + 1]);
     }
-    // key >> shift > border: taken; == border: `need` of them
-    const uint64_t differ = all ^ any;
-    int shift = differ ? 64 - __builtin_clzll(differ) : 0;
-    uint64_t border = shift < 64 ? any >> shift : 0;  // the bits that all share
-    bool whole = need == 0 || need == end - first;    // the bin is taken whole, or not at all
-    if (need == 0) {                                  // (first and last fill the list)
-        shift = 0;
-        border = ~0ull;
-        whole = false;
-    }
-    while (!whole && shift > 0 && need > 0) {
-        const int bits = min(8, shift), next = shift - bits;
-        for (int x = tid; x < 256; x += NT) hist[x] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int m = 0; m < KPT; m++) {
-            const int x = m * NT + tid;
-            if (x >= first && x < end && (shift == 64 || key[m] >> shift == border))
-                atomicAdd(&hist[(key[m] >> next) & ((1u << bits) - 1)], 1u);
+    // taken: candidates whose key is above the border's, or equal with a page up to its
+    bool done = need == 0;
+    if (need == 0) {  // first and last fill the list
+        if (tid == 0) {
+            border_key = ~0ull;
+            border_page = -1;
         }
-        __syncthreads();
-        if (w == 0) {  // the bin, from the top, that holds the need-th: lane l has bins 255 - 4l .. 252 - 4l
-            uint32_t c[4], sum = 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                c[e] = hist[255 - 4 * lane - e];
-                sum += c[e];
-            }
-            const int incl = wave_scan_i32((int)sum);
-            const uint64_t past = __ballot(incl >= need);
-            if (lane == __builtin_ctzll(past)) {
-                int above = incl - (int)sum, e = 0;
-                while (e < 3 && above + (int)c[e] < need) above += (int)c[e++];
-                pick[0] = 255 - 4 * lane - e;
-                pick[1] = need - above;
-                hist[255 - 4 * lane - e] = c[e] == (uint32_t)(need - above) ? 0xffffffffu : c[e];
-            }
-        }
-        __syncthreads();
-        const int bin = pick[0];
-        need = pick[1];
-        whole = hist[bin] == 0xffffffffu;
-        border = (shift == 64 ? 0 : border << bits) | (uint64_t)bin;
-        shift = next;
-        __syncthreads();
-    }
-    // places: a ballot per 64 pages, their counts scanned in page order
-    auto place = [&](auto taken, uint32_t (&before)[KPT]) {
-        uint64_t bal[KPT];
-#pragma unroll
-        for (int m = 0; m < KPT; m++) {
-            bal[m] = __ballot(taken(m));
-            if (lane == 0) counts[m * WAVES + w] = (uint32_t)__popcll(bal[m]);
-        }
-        __syncthreads();
-        if (w == 0) {
-            int carry = 0;
-            for (int x0 = 0; x0 < KPT * WAVES; x0 += 64) {
-                const int c = x0 + lane < KPT * WAVES ? (int)counts[x0 + lane] : 0;
-                const int incl = wave_scan_i32(c);
-                if (x0 + lane < KPT * WAVES) counts[x0 + lane] = (uint32_t)(carry + incl - c);
-                carry += __builtin_amdgcn_readlane(incl, 63);
-            }
-        }
-        __syncthreads();
+    } else if (hi > lo && hi - lo < -kNegInf) {
+        const float per = (float)BINS / (hi - lo);
+        // (monotonic; infinities and NaN keys go to the ends)
+        auto bin_of = [&](int m) { return val[m] >= hi ? BINS - 1 : val[m] <= lo ? 0 : (int)fminf((val[m] - lo) * per, BINS - 1.f); };
 #pragma unroll
         for (int m = 0; m < KPT; m++)
-            before[m] = counts[m * WAVES + w] + (uint32_t)__popcll(bal[m] & ((1ull << lane) - 1));
+            if (cand(m)) atomicAdd(&hist[bin_of(m)], 1u);
         __syncthreads();
-    };
-    uint32_t before[KPT];
-    auto cand = [&](int m) { return m * NT + tid >= first && m * NT + tid < end; };
-    auto at_border = [&](int m) { return cand(m) && (shift == 64 || key[m] >> shift == border); };
-    if (!whole) place(at_border, before);  // equal keys: the lowest pages
-    bool tie[KPT];
+        if (w == 0) find_bin(hist, BINS, need, lane, pick);
+        __syncthreads();
+        const int bin = pick[0], wanted = pick[1], held = pick[2];
+        if (held <= 64) {  // (uniform)
 #pragma unroll
-    for (int m = 0; m < KPT; m++) tie[m] = at_border(m) && (whole || before[m] < (uint32_t)need);
+            for (int m = 0; m < KPT; m++)
+                if (cand(m) && bin_of(m) == bin) {
+                    const uint32_t at = atomicAdd(&list_n, 1u);
+                    list_key[at] = key[m];
+                    list_page[at] = m * NT + tid;
+                }
+            __syncthreads();
+            if (w == 0) {  // lane l's rank among them: the `wanted`-th is the border
+                const uint64_t mine = lane < held ? list_key[lane] : 0;
+                const int page = lane < held ? list_page[lane] : INT32_MAX;
+                int rank = 0;
+                for (int x = 0; x < held; x++) {
+                    const uint64_t k = list_key[x];
+                    rank += k > mine || (k == mine && list_page[x] < page);
+                }
+                if (lane < held && rank == wanted - 1) {
+                    border_key = mine;
+                    border_page = page;
+                }
+            }
+            done = true;
+        }
+    }
+    if (!done) {
+        // radix: the key from the highest bit that differs, then the page downwards
+        uint64_t all = ~0ull, any = 0;
+#pragma unroll
+        for (int m = 0; m < KPT; m++)
+            if (cand(m)) {
+                all &= key[m];
+                any |= key[m];
+            }
+        for (int d = 32; d; d >>= 1) {
+            all &= __shfl_xor(all, d, 64);
+            any |= __shfl_xor(any, d, 64);
+        }
+        __syncthreads();
+        if (lane == 0) {
+            list_key[2 * w] = all;
+            list_key[2 * w + 1] = any;
+        }
+        __syncthreads();
+        all = ~0ull, any = 0;
+#pragma unroll
+        for (int x = 0; x < WAVES; x++) {
+            all &= list_key[2 * x];
+            any |= list_key[2 * x + 1];
+        }
+        const uint64_t differ = all ^ any;
+        int shift = differ ? 64 - __builtin_clzll(differ) : 0;
+        uint64_t top = shift < 64 ? any >> shift : 0;  // the border's bits so far
+        int page_shift = 14, page_top = 0;             // (pages < 2^14; inverted: the lowest is the largest)
+        bool whole = false;
+        auto tail = [&](int m) { return 16383 - (m * NT + tid); };
+        while (!whole && (shift > 0 || page_shift > 0)) {
+            const bool by_key = shift > 0;
+            const int bits = by_key ? min(8, shift) : 7;
+            __syncthreads();
+            for (int x = tid; x < 256; x += NT) hist[x] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int m = 0; m < KPT; m++) {
+                const bool in = cand(m) && (by_key ? (shift == 64 || key[m] >> shift == top)
+                                                   : key[m] == top && tail(m) >> page_shift == page_top);
+                const uint32_t digit = by_key ? (uint32_t)(key[m] >> (shift - bits)) : (uint32_t)tail(m) >> (page_shift - bits);
+                if (in) atomicAdd(&hist[digit & ((1u << bits) - 1)], 1u);
+            }
+            __syncthreads();
+            if (w == 0) find_bin(hist, 256, need, lane, pick);
+            __syncthreads();
+            need = pick[1];
+            whole = pick[2] == need;  // everything below this digit is taken
+            if (by_key) {
+                top = (shift == 64 ? 0 : top << bits) | (uint64_t)pick[0];
+                shift -= bits;
+            } else {
+                page_top = page_top << bits | pick[0];
+                page_shift -= bits;
+            }
+        }
+        if (tid == 0) {
+            border_key = shift < 64 ? top << shift : 0;
+            border_page = 16383 - (page_top << page_shift);
+        }
+    }
+    __syncthreads();
+    const uint64_t bk = border_key;
+    const int bp = border_page;
     auto taken = [&](int m) {
         const int x = m * NT + tid;
         if (x < first || (x >= end && x < pages)) return true;
-        return cand(m) && (tie[m] || (shift < 64 && key[m] >> shift > border));
+        return cand(m) && (key[m] > bk || (key[m] == bk && x <= bp));
     };
-    place(taken, before);
+    // places: a ballot per 64 pages, their counts scanned in page order
+    uint64_t bal[KPT];
 #pragma unroll
-    for (int m = 0; m < KPT; m++)
-        if (taken(m) && before[m] < (uint32_t)p.n_select) out[before[m]] = m * NT + tid;
+    for (int m = 0; m < KPT; m++) {
+        bal[m] = __ballot(taken(m));
+        if (lane == 0) counts[m * WAVES + w] = (uint32_t)__popcll(bal[m]);
+    }
+    __syncthreads();
+    if (w == 0) {
+        int carry = 0;
+        for (int x0 = 0; x0 < KPT * WAVES; x0 += 64) {
+            const int c = x0 + lane < KPT * WAVES ? (int)counts[x0 + lane] : 0;
+            const int incl = wave_scan_i32(c);
+            if (x0 + lane < KPT * WAVES) counts[x0 + lane] = (uint32_t)(carry + incl - c);
+            carry += __builtin_amdgcn_readlane(incl, 63);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < KPT; m++) {
+        const uint32_t at = counts[m * WAVES + w] + (uint32_t)__popcll(bal[m] & ((1ull << lane) - 1));
+        if (taken(m) && at < (uint32_t)p.n_select) out[at] = m * NT + tid;
+    }
 }
 
 template <int D>
