@@ -70,6 +70,7 @@ struct PagedDecodeParams {
     int num_splits;
     int budget;
     float scale_log2;
+    float r_mult, r_nrb, r_G, r_q_len;  // 1 / (Hk * nrb), 1 / nrb, ... for div_f
     float* ws_o;   // [B][q_len][H][num_splits][D] unnormalised partial outputs
     float* ws_ml;  // [..][2] (max in log2 units, sum)
     int* plan;
@@ -124,6 +125,13 @@ hipError_t launch_paged_decode8(const PagedDecodeParams& p, int nwg, int D, int 
 hipError_t launch_paged_combine(const PagedDecodeParams& p, int D, hipStream_t st, KernelTimer* t);
 hipError_t launch_page_score(const PageSelectParams& p, int D, int dt, hipStream_t st, KernelTimer* t);
 hipError_t launch_page_select(const PageSelectParams& p, hipStream_t st, KernelTimer* t);
+
+// n / d for 0 <= n < 2^23, rd = 1.0f / d to one ulp (a few instructions instead of
+// the 35 of an integer division)
+__device__ __forceinline__ int div_f(int n, int d, float rd) {
+    const int q = (int)((float)n * rd), r = n - q * d;
+    return r < 0 ? q - 1 : r >= d ? q + 1 : q;
+}
 
 // the physical page of a table entry, or -1
 __device__ __forceinline__ int checked_page(int id, int n_pages) { return (uint32_t)id < (uint32_t)n_pages ? id : -1; }

@@ -318,6 +318,10 @@ int decode_run(const mugen_attn_gqa_decode_paged_args* a, const DecodePlan& plan
     p.chunk = plan.chunk;
     p.num_splits = plan.splits;
     p.budget = plan.budget;
+    p.r_mult = 1.f / (float)(s.n_kv_heads * plan.nrb);
+    p.r_nrb = 1.f / (float)plan.nrb;
+    p.r_G = 1.f / (float)p.G;
+    p.r_q_len = 1.f / (float)a->q_len;
     p.scale_log2 = (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)s.head_dim)) * kLog2e;
     if (plan.splits > 1) {
         const size_t slots = (size_t)s.n_seq * a->q_len * a->n_heads * plan.splits;
@@ -325,7 +329,8 @@ int decode_run(const mugen_attn_gqa_decode_paged_args* a, const DecodePlan& plan
         p.ws_ml = p.ws_o + slots * s.head_dim;
         p.plan = reinterpret_cast<int*>(p.ws_ml + slots * 2);
     }
-    if (plan.nwg > INT32_MAX / 2 || (int64_t)p.B * p.q_len > 65535 * (int64_t)p.q_len || (int64_t)s.n_seq * a->q_len > 65535)
+    // (work items are counted in 23 bits, the merge's grid in 16)
+    if (plan.nwg >= 1 << 23 || (int64_t)s.n_seq * (s.head_dim / 64) > 65535)
         return fail(MUGEN_ATTN_E_UNSUPPORTED, "gqa_decode_paged: too many sequences or work items");
     hipError_t e = s.page_bits == 8
                        ? launch_paged_decode8(p, (int)plan.nwg, s.head_dim, s.dtype, plan.wr, st, active_timer())

@@ -68,11 +68,11 @@ __device__ __forceinline__ bool bad8(uint32_t w) { return (((w & 0x7f7f7f7fu) + 
 struct Lens {
     int T, n;
 };
+// (loads without branches, so that they leave together: what is not given is read
+// from the table, which always is there)
 __device__ __forceinline__ Lens seq_lens_of(const PagedDecodeParams& p, int b) {
-    Lens r;
-    r.T = p.seq_lens ? clamp_len(p.seq_lens[b], p.st.max_T) : p.fixed_T;
-    r.n = p.q_lens ? min(max(p.q_lens[b], 0), p.q_len) : p.q_len;
-    return r;
+    const int T = *(p.seq_lens ? p.seq_lens + b : p.st.table), n = *(p.q_lens ? p.q_lens + b : p.st.table);
+    return Lens{p.seq_lens ? clamp_len(T, p.st.max_T) : p.fixed_T, p.q_lens ? clamp_len(n, p.q_len) : p.q_len};
 }
 
 // list entries a query that sees `limit` tokens may use
@@ -84,13 +84,18 @@ __device__ __forceinline__ int list_len(const PagedDecodeParams& p, int limit) {
 template <bool LIST>
 __device__ __forceinline__ int range_of(const PagedDecodeParams& p, int j) {
     if constexpr (LIST) {
-        const int b = j / p.q_len, i = j - b * p.q_len;
+        const int b = div_f(j, p.q_len, p.r_q_len), i = j - b * p.q_len;
         const Lens s = seq_lens_of(p, b);
         return i < s.n ? list_len(p, s.T - s.n + i + 1) << p.st.p_shift : 0;
     } else {
         const Lens s = seq_lens_of(p, j);
         return s.n > 0 ? s.T : 0;
     }
+}
+
+// splits of a key range of `len` tokens, chunks of `units` 32-token tiles
+__device__ __forceinline__ int splits_of(int len, int units, float r_units) {
+    return ceil_div_f((len + 31) >> 5, units, r_units);
 }
 
 template <bool LIST>
@@ -120,25 +125,31 @@ __global__ __launch_bounds__(64 * WR * paged_tiles(D, BITS8, WR))
     __shared__ __attribute__((aligned(16))) char lds[STAGE > MERGE ? STAGE : MERGE];
 
     const int Hk = p.st.Hk, ps = p.st.p_shift, P = 1 << ps;
+    // one sequence, planned by the host: the split's place is known without the length,
+    // so its page ids are on their way meanwhile
+    const bool early = !LIST && p.B == 1 && p.chunk;
+    int early_id = -1;
+    if (early) {
+        const int page = (div_f((int)blockIdx.x, Hk * p.nrb, p.r_mult) * p.chunk >> ps) + (int)(threadIdx.x & 63);
+        early_id = p.st.table[min(page, (p.st.max_T - 1) >> ps)];
+    }
     const int chunk = p.chunk ? p.chunk : plan<LIST>(p);
     int j = -1, r = 0;
     const int mult = Hk * p.nrb;
-    auto items = [&](int x) {
-        const int len = range_of<LIST>(p, x);
-        return (len > 0 ? (len + chunk - 1) / chunk : 1) * mult;
-    };
+    const float r_units = plan_rcp(chunk >> 5);
+    auto items = [&](int x) { return max(1, splits_of(range_of<LIST>(p, x), chunk >> 5, r_units)) * mult; };
     if (!find_sequence(p.B, (int)blockIdx.x, items, j, r)) return;  // grid padding
-    const int s = r / mult, kr = r - s * mult, kvh = kr / p.nrb, rb = kr - kvh * p.nrb;
+    const int s = div_f(r, mult, p.r_mult), kr = r - s * mult, kvh = div_f(kr, p.nrb, p.r_nrb), rb = kr - kvh * p.nrb;
     if (p.num_splits > 1 && s >= p.num_splits) return;  // past the workspace's stride
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int b = LIST ? j / p.q_len : j, i0 = LIST ? j - b * p.q_len : 0;
+    const int b = LIST ? div_f(j, p.q_len, p.r_q_len) : j, i0 = LIST ? j - b * p.q_len : 0;
     const Lens len = seq_lens_of(p, b);
     const int T = len.T;
     const int range = range_of<LIST>(p, j);
     const int t_begin = s * chunk, t_end = min(t_begin + chunk, range);
     if (p.chunk == 0 && blockIdx.x == 0 && threadIdx.x == 0) *p.plan = chunk;  // for the merge
-    const int n_act = min(p.num_splits, max(1, (range + chunk - 1) / chunk));  // splits of this range
+    const int n_act = min(p.num_splits, max(1, splits_of(range, chunk >> 5, r_units)));  // splits of this range
     const int G = p.G, wg_row = rb * WR * 16, n_rows = (LIST ? 1 : len.n) * G;
     if (wg_row >= n_rows) return;  // rows of tokens that are not there
     const int wr = w % WR, wt = w / WR, first_row = wg_row + 16 * wr;
@@ -146,7 +157,7 @@ __global__ __launch_bounds__(64 * WR * paged_tiles(D, BITS8, WR))
     // the lane's row first_row + n: its query, and how many tokens that sees
     const int row = first_row + n;
     const bool live = row < n_rows;
-    const int tok = LIST ? i0 : row / G;
+    const int tok = LIST ? i0 : div_f(row, G, p.r_G);
     const int limit = live ? max(T - len.n + tok + 1, 0) : 0;
     u32x4_t qf[KK];
     {
@@ -156,7 +167,8 @@ __global__ __launch_bounds__(64 * WR * paged_tiles(D, BITS8, WR))
             qf[kk] = live ? load16(qp + 64 * (kk >> 1) + 16 * g + 8 * (kk & 1)) : u32x4_t{0, 0, 0, 0};
     }
     // the wave's first and last token; tiles below `low` are seen by all its rows
-    const int tok_first = LIST ? i0 : first_row / G, tok_last = LIST ? i0 : (min(first_row + 16, n_rows) - 1) / G;
+    const int tok_first = LIST ? i0 : div_f(first_row, G, p.r_G),
+              tok_last = LIST ? i0 : div_f(min(first_row + 16, n_rows) - 1, G, p.r_G);
     const int low = first_row < n_rows ? max(T - len.n + tok_first + 1, 0) : 0;
     const int t_first = first_row < n_rows ? t_begin + 32 * wt : t_end;  // (a wave without rows has no tiles)
 
@@ -187,7 +199,8 @@ __global__ __launch_bounds__(64 * WR * paged_tiles(D, BITS8, WR))
                 if (lp <= before || lp >= (my_limit + P - 1) >> ps) lp = -1;
             }
             if (lp >= 0) {
-                if (!BITS8 || lp < whole) x.phys = checked_page(table[lp], p.st.n_pages);
+                if (!BITS8 || lp < whole)
+                    x.phys = checked_page(early && page0 == first_page ? early_id : table[lp], p.st.n_pages);
                 x.lp = lp;
             }
         }
@@ -554,7 +567,7 @@ __global__ __launch_bounds__(64 * WR * paged_tiles(D, BITS8, WR))
     const int rows_here = min(WR * 16, n_rows - wg_row);
     // row r of the workgroup in q and out
     auto out_row = [&](int r2) {
-        const int i = LIST ? i0 : (wg_row + r2) / G;
+        const int i = LIST ? i0 : div_f(wg_row + r2, G, p.r_G);
         return ((int64_t)b * p.q_len + i) * p.H + kvh * G + (LIST ? r2 : wg_row + r2 - i * G);
     };
     auto store4 = [&](int64_t orow, int d, f32x4_t v) {
@@ -573,18 +586,16 @@ __global__ __launch_bounds__(64 * WR * paged_tiles(D, BITS8, WR))
         for (int x = 0; x < WT; x++) {
             const int at = (x * WR + (h >> 4)) * 16 + (h & 15);
             const float f = f_lds[at];
-            if (f != 0.f) O += f * *reinterpret_cast<const f32x4_t*>(&o_lds[at * OROW + d]);
+            const f32x4_t v = *reinterpret_cast<const f32x4_t*>(&o_lds[at * OROW + d]);
+            O += f * (f != 0.f ? v : f32x4_t{0.f, 0.f, 0.f, 0.f});
         }
         const int64_t orow = out_row(h);
         if (n_act == 1) {
             store4(orow, d, O);
         } else {
             const int64_t slot = orow * p.num_splits + s;
-            store_wt(reinterpret_cast<u32x4_t*>(p.ws_o + slot * D + d), __builtin_bit_cast(u32x4_t, O));
-            if (d == 0) {
-                store_wt(p.ws_ml + slot * 2, ml_out[2 * h]);
-                store_wt(p.ws_ml + slot * 2 + 1, ml_out[2 * h + 1]);
-            }
+            *reinterpret_cast<f32x4_t*>(p.ws_o + slot * D + d) = O;
+            if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = float2{ml_out[2 * h], ml_out[2 * h + 1]};
         }
     }
 }

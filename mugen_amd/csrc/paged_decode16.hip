@@ -10,15 +10,17 @@ template <int D, bool LIST>
 __global__ __launch_bounds__(64) void paged_combine_kernel(PagedDecodeParams p) {
     constexpr int kPre = 32;
     __shared__ float f_lds[64];
-    const int h = blockIdx.x, d = blockIdx.z * 64 + threadIdx.x, lane = threadIdx.x;
-    const int b = (int)blockIdx.y / p.q_len, i = (int)blockIdx.y - b * p.q_len;
+    // grid (H, q_len, B * D / 64): no division before the loads
+    const int h = blockIdx.x, i = blockIdx.y, b = (int)blockIdx.z / (D / 64), lane = threadIdx.x;
+    const int d = (int)blockIdx.z % (D / 64) * 64 + lane;
+    const int planned = *p.plan;
     const paged::Lens len = paged::seq_lens_of(p, b);
     if (i >= len.n) return;  // no such token: its row stays as it was
-    const int chunk = p.chunk ? p.chunk : *p.plan;
-    const int range = paged::range_of<LIST>(p, LIST ? (int)blockIdx.y : b);
-    const int nact = min(p.num_splits, (range + chunk - 1) / chunk);
+    const int units = (p.chunk ? p.chunk : planned) >> 5;
+    const int range = LIST ? paged::list_len(p, len.T - len.n + i + 1) << p.st.p_shift : len.T;
+    const int nact = min(p.num_splits, paged::splits_of(range, units, plan_rcp(units)));
     if (nact <= 1) return;  // one split: the result is there
-    const int64_t row = (int64_t)blockIdx.y * p.H + h;
+    const int64_t row = ((int64_t)b * p.q_len + i) * p.H + h;
     const float* ml = p.ws_ml + row * p.num_splits * 2;
     const float* os = p.ws_o + row * p.num_splits * D + d;
     float M = kNegInf, L = 0.f, O = 0.f;
@@ -38,17 +40,20 @@ __global__ __launch_bounds__(64) void paged_combine_kernel(PagedDecodeParams p) 
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        // (a weight of 0, also that of lanes past the splits, keeps out what its
+        // partial may be; no branch, so the weights' LDS reads overlap)
+        float acc[4] = {O, 0.f, 0.f, 0.f};
+        auto add = [&](int k, float weight, float x) { acc[k & 3] = fmaf(weight, weight != 0.f ? x : 0.f, acc[k & 3]); };
 #pragma unroll
-        for (int k = 0; k < kPre; k++)
-            if (k < ns && f_lds[k] != 0.f) O += f_lds[k] * v[k];
-        for (int s = kPre; s < ns; s += 8) {
-            float u[8];
+        for (int k = 0; k < kPre; k++) add(k, f_lds[k], v[k]);
+        for (int s = kPre; s < ns; s += 16) {
+            float u[16];
 #pragma unroll
-            for (int k = 0; k < 8; k++) u[k] = os[(int64_t)(s0 + min(s + k, ns - 1)) * D];
+            for (int k = 0; k < 16; k++) u[k] = os[(int64_t)(s0 + min(s + k, ns - 1)) * D];
 #pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (s + k < ns && f_lds[s + k] != 0.f) O += f_lds[s + k] * u[k];
+            for (int k = 0; k < 16; k++) add(k, f_lds[s + k], u[k]);
         }
+        O = (acc[0] + acc[1]) + (acc[2] + acc[3]);
         __builtin_amdgcn_wave_barrier();
     }
     O = L > 0.f ? O / L : L == L ? 0.f : L;
@@ -59,7 +64,7 @@ __global__ __launch_bounds__(64) void paged_combine_kernel(PagedDecodeParams p) 
 
 template <int D>
 static hipError_t launch_combine_d(const PagedDecodeParams& p, hipStream_t st, KernelTimer* t) {
-    const dim3 grid(p.H, p.sel ? p.B : p.B * p.q_len, D / 64);
+    const dim3 grid(p.H, p.q_len, (p.sel ? p.B / p.q_len : p.B) * (D / 64));
     if (p.sel) return launch_k(t, "gqa_decode_paged_combine", paged_combine_kernel<D, true>, grid, dim3(64), st, p);
     return launch_k(t, "gqa_decode_paged_combine", paged_combine_kernel<D, false>, grid, dim3(64), st, p);
 }
