@@ -861,7 +861,19 @@ size_t mugen_attn_gqa_prefill_workspace_size(const mugen_attn_gqa_prefill_args* 
     return (gqa_prefill_uses_v16(a) ? gqa_prefill_ws(a) : 0) + gqa_prefill_split(a).bytes;
 }
 
-int mugen_attn_gqa_prefill(const mugen_attn_gqa_prefill_args* a, void* stream) {
+int mugen_attn_gqa_prefill(const mugen_attn_gqa_prefill_args* a, void* stream) { return prefill_run(a, false, stream); }
+
+}  // extern "C"
+
+namespace mugen_attn {
+
+bool prefill_takes_v16(const mugen_attn_gqa_prefill_args* a) { return gqa_prefill_uses_v16(a) && !gqa_prefill_short_default(a); }
+
+size_t prefill_split_workspace(const mugen_attn_gqa_prefill_args* a) { return gqa_prefill_split(a).bytes; }
+
+// v16: a->v already is the fp16 copy (prefill_takes_v16), the workspace the
+// split partials' alone
+int prefill_run(const mugen_attn_gqa_prefill_args* a, bool v16, void* stream) {
     if (int rc = gqa_prefill_validate(a)) return rc;
     if (a->n_tokens == 0) return MUGEN_ATTN_OK;
     GqaPrefillParams p{};
@@ -933,8 +945,8 @@ int mugen_attn_gqa_prefill(const mugen_attn_gqa_prefill_args* a, void* stream) {
         return fail(MUGEN_ATTN_E_UNSUPPORTED,
                     "gqa_prefill: the short kernel serves head_dim 64, n_heads/n_kv_heads <= 4 and <= 512 keys");
     if (a->kernel) kernel = a->kernel;
-    int dt = a->dtype;
-    const size_t v16_bytes = gqa_prefill_uses_v16(a) ? gqa_prefill_ws(a) : 0;
+    int dt = v16 ? kDtBf16V16 : a->dtype;
+    const size_t v16_bytes = gqa_prefill_uses_v16(a) && !v16 ? gqa_prefill_ws(a) : 0;
     const PrefillSplit split = gqa_prefill_split(a);  // none for the short kernel (default or forced)
     p.ksplit = 1;
     if (split.ksplit > 1 && a->workspace && a->workspace_bytes >= v16_bytes + split.bytes) {
@@ -962,6 +974,10 @@ int mugen_attn_gqa_prefill(const mugen_attn_gqa_prefill_args* a, void* stream) {
                                             static_cast<hipStream_t>(stream), active_timer());
     return hip_status(e, "gqa_prefill launch");
 }
+
+}  // namespace mugen_attn
+
+extern "C" {
 
 size_t mugen_attn_mla_decode_workspace_size(const mugen_attn_mla_decode_args* a) {
     if (mla_validate(a) != MUGEN_ATTN_OK) return 0;

@@ -356,7 +356,12 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(PagedGatherParams p) 
         for (int i = threadIdx.x; i < n * (D / 8); i += 256) {
             const int r = i / (D / 8), d = 8 * (i % (D / 8));
             *reinterpret_cast<u32x4_t*>(ko + r * row + d) = ks ? load16(ks + r * srow + d) : u32x4_t{0, 0, 0, 0};
-            *reinterpret_cast<u32x4_t*>(vo + r * row + d) = ks ? load16(vs + r * srow + d) : u32x4_t{0, 0, 0, 0};
+            u32x4_t v = ks ? load16(vs + r * srow + d) : u32x4_t{0, 0, 0, 0};
+            if (DT == DT_BF16 && p.v16) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = pack2<DT_F16>(lo_f32<DT>(v[e]), hi_f32<DT>(v[e]));
+            }
+            *reinterpret_cast<u32x4_t*>(vo + r * row + d) = v;
         }
         return;
     }
@@ -374,7 +379,8 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(PagedGatherParams p) 
             const int d = i >> 1, r = 16 * (i & 1);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const u32x4_t y = cvt8_fp8<DT>(x[2 * h], x[2 * h + 1], sv);
+                const u32x4_t y = DT == DT_F16 || p.v16 ? cvt8_fp8<DT_F16>(x[2 * h], x[2 * h + 1], sv)
+                                                        : cvt8_fp8<DT>(x[2 * h], x[2 * h + 1], sv);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     tile[(r + 8 * h + 2 * e) * (D + 8) + d] = (uint16_t)y[e];

@@ -113,6 +113,7 @@ struct PagedGatherParams {
     uint16_t* v_out;
     int seq;
     int T;
+    int v16;  // V in fp16 whatever the store's type
 };
 
 hipError_t launch_paged_append(PagedAppendParams p, const RopeTurns<128>& turns, int D, int dt, bool bits8, hipStream_t st, KernelTimer* t);

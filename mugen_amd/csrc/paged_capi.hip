@@ -453,9 +453,16 @@ mugen_attn_gqa_prefill_args gathered(const mugen_attn_gqa_prefill_paged_args* a,
     return g;
 }
 
-// Few tokens go through the decode kernel, which reads the pages as they are
+// Few tokens go through the decode kernel, which reads the pages as they are; more
+// of them through the gathered rows, which cost their copy but feed the prompt
+// kernels (us rows / gathered, 8-bit pages; 28 / 4 heads d128, 112 / 168 / 224 rows a kv
+// head: after 1k 11.2 / 14.6, 12.9 / 14.7, 14.5 / 14.9, after 8k 17.6 / 21.8, 24.3 / 22.5,
+// 24.6 / 22.9, after 32k 35 / 47, 45 / 48, 58 / 48; 32 / 8 d64, 256 rows: 12.8 / 11.8,
+// 22.4 / 24.1, 47 / 58; 16 / 8 d256, 128 rows: 21.5 / 26.1, 40 / 61, 123 / 155)
+constexpr int kRowsMost = 160, kRowsMostOther = 256;  // head_dim 128; 64 and 256
 bool prefill_by_rows(const mugen_attn_gqa_prefill_paged_args* a) {
-    return a->n_tokens <= MUGEN_ATTN_PAGED_MAX_Q && a->n_tokens * (a->n_heads / a->store.n_kv_heads) <= 64;
+    return a->n_tokens <= MUGEN_ATTN_PAGED_MAX_Q &&
+           a->n_tokens * (a->n_heads / a->store.n_kv_heads) <= (a->store.head_dim == 128 ? kRowsMost : kRowsMostOther);
 }
 mugen_attn_gqa_decode_paged_args as_decode(const mugen_attn_gqa_prefill_paged_args* a, int32_t* len) {
     mugen_attn_gqa_decode_paged_args d{};
@@ -487,7 +494,7 @@ extern "C" size_t mugen_attn_gqa_prefill_paged_workspace_size(const mugen_attn_g
         return decode_plan(&d, true).bytes;
     }
     const mugen_attn_gqa_prefill_args g = gathered(a, a->store.k_pages, a->store.v_pages);
-    return 256 + 2 * gather_bytes(a) + mugen_attn_gqa_prefill_workspace_size(&g);
+    return 256 + 2 * gather_bytes(a) + prefill_split_workspace(&g);
 }
 
 extern "C" int mugen_attn_gqa_prefill_paged(const mugen_attn_gqa_prefill_paged_args* a, void* ws, size_t ws_bytes,
@@ -510,14 +517,15 @@ extern "C" int mugen_attn_gqa_prefill_paged(const mugen_attn_gqa_prefill_paged_a
     p.v_out = reinterpret_cast<uint16_t*>(base + gather_bytes(a));
     p.seq = a->seq;
     p.T = a->start_pos + a->n_tokens;
+    mugen_attn_gqa_prefill_args g = gathered(a, p.k_out, p.v_out);
+    p.v16 = prefill_takes_v16(&g);
     if (int rc = hip_status(launch_paged_gather(p, a->store.head_dim, a->store.dtype, a->store.page_bits == 8, st, active_timer()),
                             "gqa_prefill_paged launch"))
         return rc;
-    mugen_attn_gqa_prefill_args g = gathered(a, p.k_out, p.v_out);
-    const size_t more = mugen_attn_gqa_prefill_workspace_size(&g);
+    const size_t more = prefill_split_workspace(&g);
     if (more) {
         g.workspace = base + 2 * gather_bytes(a);
         g.workspace_bytes = more;
     }
-    return mugen_attn_gqa_prefill(&g, stream);
+    return prefill_run(&g, p.v16, stream);
 }
