@@ -86,7 +86,7 @@ __host__ __device__ constexpr int paged_waves_per_simd(int D, bool bits8) {
 // A workgroup: WR waves take a tile's 16-row blocks side by side, paged_tiles tiles
 // are under way.  4 waves in all, one to a SIMD, or 12 (three row blocks), which
 // fill a CU that holds 3 to a SIMD (two workgroups of 6 do not fit beside each other:
-// 2, 2, 1, 1 waves each; 5 drafted tokens of 28 / 4 heads over 4 x 31k 47 -> 35 us)
+// 2, 2, 1, 1 waves each; 5 drafted tokens of 28 / 4 heads over 4 x 31k 46.7 -> 37.7 us)
 __host__ __device__ constexpr int paged_tiles(int D, bool bits8, int WR) {
     return WR == 1 ? 4 : WR == 2 ? 2 : WR == 4 ? 1 : paged_waves_per_simd(D, bits8) >= 3 ? 4 : 2;
 }

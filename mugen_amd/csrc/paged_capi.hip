@@ -455,11 +455,11 @@ mugen_attn_gqa_prefill_args gathered(const mugen_attn_gqa_prefill_paged_args* a,
 
 // Few tokens go through the decode kernel, which reads the pages as they are; more
 // of them through the gathered rows, which cost their copy but feed the prompt
-// kernels (us rows / gathered, 8-bit pages; 28 / 4 heads d128, 112 / 168 / 224 rows a kv
-// head: after 1k 11.2 / 14.6, 12.9 / 14.7, 14.5 / 14.9, after 8k 17.6 / 21.8, 24.3 / 22.5,
-// 24.6 / 22.9, after 32k 35 / 47, 45 / 48, 58 / 48; 32 / 8 d64, 256 rows: 12.8 / 11.8,
-// 22.4 / 24.1, 47 / 58; 16 / 8 d256, 128 rows: 21.5 / 26.1, 40 / 61, 123 / 155)
-constexpr int kRowsMost = 160, kRowsMostOther = 256;  // head_dim 128; 64 and 256
+// kernels (us rows / gathered, 8-bit pages; 28 / 4 heads d128, 168 / 224 / 336 rows a kv
+// head: after 1k 12.9 / 14.7, 14.0 / 15.0, 18.8 / 15.1, after 8k 22.8 / 22.4, 24.1 / 22.9,
+// 29.5 / 33.4, after 32k 38 / 48, 45 / 49, 57 / 79; 32 / 8 d64, 256 rows: 12.8 / 11.8,
+// 23.3 / 24.1, 44 / 58; 16 / 8 d256, 128 rows: 21.0 / 26.1, 36 / 61, 89 / 155)
+constexpr int kRowsMost = 224, kRowsMostOther = 256;  // head_dim 128; 64 and 256
 bool prefill_by_rows(const mugen_attn_gqa_prefill_paged_args* a) {
     return a->n_tokens <= MUGEN_ATTN_PAGED_MAX_Q &&
            a->n_tokens * (a->n_heads / a->store.n_kv_heads) <= (a->store.head_dim == 128 ? kRowsMost : kRowsMostOther);
