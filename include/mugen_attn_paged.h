@@ -94,9 +94,10 @@ typedef struct mugen_attn_kv_pages {
  * phase, the result is rounded to dtype once.
  * With page_bits 8 the pages that these tokens fill are quantised, from the ring
  * and the new rows, and the newest `ring` new rows go to the ring.  After a step whose
- * last tokens are rejected, seq_lens may go back by up to
- * ring - page_tokens tokens (and never behind a ring-ful): appends write
- * the same pages again.  Requires rope_dim a multiple of 16 up to head_dim.
+ * last tokens are rejected, seq_lens may go back, as long as the rows of the page
+ * that is open then are still in the ring (it holds the last `ring` positions ever
+ * written, so any ring - page_tokens tokens behind the furthest): appends write the
+ * same pages again.  Requires rope_dim a multiple of 16 up to head_dim.
  */
 typedef struct mugen_attn_kv_paged_append_args {
     mugen_attn_kv_pages store;

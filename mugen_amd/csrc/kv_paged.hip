@@ -91,34 +91,54 @@ __device__ __forceinline__ void append_rows(const PagedAppendParams& p, const Ro
     unit_dims(u, p.rope_dim, d0, d1);
     const bool rot = 16 * u < p.rope_dim;
     const int h_end = min((hg + 1) * hpt, heads);
+    // where the token's K and V rows go (heads kv_head elements apart; -1: nowhere)
+    int64_t kv_at = -1, kv_head = D;
+    uint16_t *k_to, *v_to;
+    if constexpr (BITS8) {
+        k_to = p.st.tail_k;
+        v_to = p.st.tail_v;
+        // (not if this call's own tokens push it out of the ring)
+        if (pos >= T_out - p.st.ring && !page_jobs_slot(p, T, T_out, pos))
+            kv_at = b * p.st.tail_stride + (int64_t)(pos & (p.st.ring - 1)) * p.st.Hk * D;
+    } else {
+        k_to = reinterpret_cast<uint16_t*>(p.st.k);
+        v_to = reinterpret_cast<uint16_t*>(p.st.v);
+        const int page = checked_page(p.st.table[b * p.st.table_stride + (pos >> p.st.p_shift)], p.st.n_pages);
+        kv_head = (int64_t)D << p.st.p_shift;
+        if (page >= 0) kv_at = (int64_t)page * p.st.Hk * kv_head + (pos & ((1 << p.st.p_shift) - 1)) * D;
+    }
     Turn8 turn{};
     if (rot && hg * hpt < p.H + p.st.Hk) turn = turn8(turns, u, pos);  // (V heads come last)
-    for (int h = hg * hpt; h < h_end; h++) {
-        const uint16_t* src;
-        uint16_t* dst;
-        if (h < p.H) {
-            src = p.q + id * p.q_stride + (int64_t)h * D;
-            dst = p.q_out + (id * p.H + h) * D;
-        } else {
-            const bool is_v = h >= p.H + p.st.Hk;
-            const int kvh = h - p.H - (is_v ? p.st.Hk : 0);
-            src = (is_v ? p.v_new + id * p.v_stride : p.k_new + id * p.k_stride) + (int64_t)kvh * D;
-            if constexpr (BITS8) {
-                if (pos < T_out - p.st.ring) continue;  // pushed out of the ring by this call's own tokens
-                if (page_jobs_slot(p, T, T_out, pos)) continue;
-                dst = (is_v ? p.st.tail_v : p.st.tail_k) + b * p.st.tail_stride +
-                      ((int64_t)(pos & (p.st.ring - 1)) * p.st.Hk + kvh) * D;
+    // four heads at a time: their rows are all on the way before the first is turned
+    for (int h0 = hg * hpt; h0 < h_end; h0 += 4) {
+        u32x4_t x[4], y[4];
+        uint16_t* to[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int h = h0 + e;
+            const uint16_t* src;
+            to[e] = nullptr;
+            if (h >= h_end) continue;
+            if (h < p.H) {
+                src = p.q + id * p.q_stride + (int64_t)h * D;
+                to[e] = p.q_out + (id * p.H + h) * D;
             } else {
-                const int page = checked_page(p.st.table[b * p.st.table_stride + (pos >> p.st.p_shift)], p.st.n_pages);
-                if (page < 0) continue;
-                dst = reinterpret_cast<uint16_t*>(is_v ? p.st.v : p.st.k) +
-                      ((((int64_t)page * p.st.Hk + kvh) << p.st.p_shift) + (pos & ((1 << p.st.p_shift) - 1))) * D;
+                const bool is_v = h >= p.H + p.st.Hk;
+                const int kvh = h - p.H - (is_v ? p.st.Hk : 0);
+                src = (is_v ? p.v_new + id * p.v_stride : p.k_new + id * p.k_stride) + (int64_t)kvh * D;
+                if (kv_at >= 0) to[e] = (is_v ? v_to : k_to) + kv_at + (int64_t)kvh * kv_head;
             }
+            if (!to[e]) continue;
+            x[e] = load16(src + d0);
+            y[e] = load16(src + d1);
         }
-        u32x4_t x = load16(src + d0), y = load16(src + d1);
-        if (rot && h < p.H + p.st.Hk) rotate8<DT>(turn, x, y);
-        *reinterpret_cast<u32x4_t*>(dst + d0) = x;
-        *reinterpret_cast<u32x4_t*>(dst + d1) = y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (!to[e]) continue;
+            if (rot && h0 + e < p.H + p.st.Hk) rotate8<DT>(turn, x[e], y[e]);
+            *reinterpret_cast<u32x4_t*>(to[e] + d0) = x[e];
+            *reinterpret_cast<u32x4_t*>(to[e] + d1) = y[e];
+        }
     }
 }
 

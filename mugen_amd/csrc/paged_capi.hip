@@ -164,7 +164,7 @@ extern "C" int mugen_attn_kv_paged_append(const mugen_attn_kv_paged_append_args*
     const int64_t tokens = (int64_t)s.n_seq * a->n_new;
     // one head a thread where the tokens are few (latency), up to 8 where their
     // threads fill the card anyway (the sines are shared)
-    p.heads_per_thread = (int)std::min<int64_t>(8, std::max<int64_t>(1, tokens * heads * (s.head_dim / 16) / (256 * 1024)));
+    p.heads_per_thread = (int)std::min<int64_t>(8, std::max<int64_t>(1, tokens * heads * (s.head_dim / 16) / (64 * 1024)));
     p.pages = (a->n_new + s.page_tokens - 1) / s.page_tokens;  // that n_new tokens can fill
     const int64_t jobs = (int64_t)s.n_seq * p.pages * s.n_kv_heads * 2;
     if (tokens * heads * (s.head_dim / 16) > INT32_MAX || jobs > INT32_MAX / 2)
@@ -187,20 +187,19 @@ struct DecodePlan {
     size_t bytes = 0;
 };
 
-// the key ranges the plan cuts: sequences, or (with page lists) queries
+// the key ranges the plan cuts: sequences, or (with page lists) queries, whose lists
+// are as long as the last query's at most
 int ranges_of(const mugen_attn_gqa_decode_paged_args* a) { return a->store.n_seq * (a->pages ? a->q_len : 1); }
-int64_t longest_range(const mugen_attn_gqa_decode_paged_args* a) {
-    const int64_t T = a->store.max_seq_len;
+int64_t range_of_len(const mugen_attn_gqa_decode_paged_args* a, int T) {
     if (!a->pages) return T;
-    const int64_t P = a->store.page_tokens;
-    return std::min<int64_t>((int64_t)a->n_select, ceil_div(T, P)) * P;
+    const int P = a->store.page_tokens;
+    return (int64_t)std::min((uint32_t)a->n_select, ((uint32_t)T + P - 1) / P) * P;
 }
-int64_t range_len(const mugen_attn_gqa_decode_paged_args* a, int x) {
+int64_t longest_range(const mugen_attn_gqa_decode_paged_args* a) { return range_of_len(a, a->store.max_seq_len); }
+// of sequence b
+int64_t range_len(const mugen_attn_gqa_decode_paged_args* a, int b) {
     if (!a->seq_lens_host) return longest_range(a);
-    const int64_t T = std::min(std::max(a->seq_lens_host[a->pages ? x / a->q_len : x], 0), a->store.max_seq_len);
-    if (!a->pages) return T;
-    const int64_t P = a->store.page_tokens;
-    return std::min<int64_t>((int64_t)a->n_select, ceil_div(T, P)) * P;  // (an earlier query sees no more)
+    return range_of_len(a, std::min(std::max(a->seq_lens_host[b], 0), a->store.max_seq_len));
 }
 
 // most splits of a range: 32, more only in pieces of 512 tokens and up
@@ -208,12 +207,14 @@ constexpr int kCap = 32, kCapLong = kPagedMaxSplits, kCapTokens = 512, kChunkMin
 int split_cap(int64_t len) { return (int)std::max<int64_t>(kCap, std::min<int64_t>(kCapLong, len / kCapTokens)); }
 int split_bound(int64_t len) { return (int)std::min<int64_t>(split_cap(len), ceil_div(len, kChunkMin)); }
 
-int64_t decode_items(const mugen_attn_gqa_decode_paged_args* a, int chunk, int64_t mult) {
+// work items of a chunk size; counting ends past `most` (the search asks no more)
+int64_t decode_items(const mugen_attn_gqa_decode_paged_args* a, int chunk, int64_t mult, int64_t most = INT64_MAX) {
+    if (!a->seq_lens_host) return ranges_of(a) * std::max<int64_t>(1, ceil_div(longest_range(a), chunk)) * mult;
+    const int64_t each = mult * (a->pages ? a->q_len : 1);
     int64_t n = 0;
-    const int R = ranges_of(a);
-    if (!a->seq_lens_host) return R * std::max<int64_t>(1, ceil_div(longest_range(a), chunk)) * mult;
-    for (int x = 0; x < R; x++) n += std::max<int64_t>(1, ceil_div(range_len(a, x), chunk));
-    return n * mult;
+    for (int b = 0; b < a->store.n_seq && n * each <= most; b++)
+        n += std::max(1u, ((uint32_t)range_len(a, b) + chunk - 1) / (uint32_t)chunk);
+    return n * each;
 }
 
 size_t decode_bytes(const mugen_attn_gqa_decode_paged_args* a, int splits) {
@@ -232,17 +233,17 @@ DecodePlan decode_plan(const mugen_attn_gqa_decode_paged_args* a, bool for_size)
     r.budget = 256 * paged_groups_per_cu(s.head_dim, s.page_bits == 8, r.wr);
     const int64_t longest = longest_range(a);
     int64_t len = 1;
-    for (int x = 0, R = a->seq_lens_host ? ranges_of(a) : 1; x < R; x++) len = std::max(len, range_len(a, x));
+    for (int b = 0, B = a->seq_lens_host ? s.n_seq : 1; b < B; b++) len = std::max(len, range_len(a, b));
     if (a->num_splits > 0) {
         r.chunk = (int)ceil_div(ceil_div(longest, a->num_splits), 32) * 32;
     } else {
         const int64_t most = ceil_div(len, 32) * 32;
         int64_t lo = std::max<int64_t>(ceil_div(ceil_div(len, split_cap(len)), 32) * 32, kChunkMin), hi = std::max(most, lo);
-        if (decode_items(a, (int)hi, mult) > r.budget) lo = hi;  // a range each already fills the round
+        if (decode_items(a, (int)hi, mult, r.budget) > r.budget) lo = hi;  // a range each already fills the round
         while (lo < hi) {                                        // items fall as the chunk grows
             const int64_t mid = (lo + hi) / 2 / 32 * 32;
             if (mid < lo) break;
-            if (decode_items(a, (int)mid, mult) <= r.budget) hi = mid;
+            if (decode_items(a, (int)mid, mult, r.budget) <= r.budget) hi = mid;
             else lo = mid + 32;
         }
         r.chunk = (int)hi;
@@ -250,7 +251,7 @@ DecodePlan decode_plan(const mugen_attn_gqa_decode_paged_args* a, bool for_size)
         // the longest range would run on alone
         if (a->seq_lens_host && r.chunk > 1024) {
             int64_t sum = 0;
-            for (int x = 0; x < ranges_of(a); x++) sum += range_len(a, x);
+            for (int b = 0; b < s.n_seq; b++) sum += range_len(a, b) * (a->pages ? a->q_len : 1);
             if ((double)std::min<int64_t>(r.chunk, len) * r.budget > 1.35 * (double)(sum * mult))
                 r.chunk = (int)std::max<int64_t>(1024, ceil_div(ceil_div(len, kCap), 32) * 32);
         }
@@ -279,7 +280,8 @@ int decode_validate(const mugen_attn_gqa_decode_paged_args* a) {
     if (int rc = store_validate(a->store, who)) return rc;
     if (int rc = heads_validate(a->store, a->n_heads, who)) return rc;
     if (!a->q || !a->out || !a->seq_lens) return fail(MUGEN_ATTN_E_INVALID, "%s: null tensor pointer", who);
-    if (!aligned16(a->q)) return fail(MUGEN_ATTN_E_INVALID, "%s: q must be 16-byte aligned", who);
+    if (!aligned16(a->q) || !aligned16(a->out))
+        return fail(MUGEN_ATTN_E_INVALID, "%s: q and out must be 16-byte aligned", who);
     if (a->q_len <= 0 || a->q_len > MUGEN_ATTN_PAGED_MAX_Q)
         return fail(MUGEN_ATTN_E_UNSUPPORTED, "%s: q_len %d (supported: 1 .. %d)", who, a->q_len, MUGEN_ATTN_PAGED_MAX_Q);
     if (a->num_splits < 0 || a->num_splits > kPagedMaxSplits)

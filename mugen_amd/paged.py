@@ -76,6 +76,16 @@ _current_device = getattr(torch._C, "_cuda_getDevice", lambda: -1)
 _i32 = torch.int32
 
 
+def _host_address(lens, n_seq: int):
+    """Address of an int32 host copy of the lengths, and what keeps it alive."""
+    lens = np.ascontiguousarray(lens, np.int32)
+    if lens.size != n_seq:
+        raise ValueError("seq_lens_host must have one entry per sequence")
+    if not lens.flags.writeable:  # (a ctypes view of it is refused)
+        lens = lens.copy()
+    return ctypes.addressof(ctypes.c_char.from_buffer(lens)), lens  # (a quarter of the time of lens.ctypes.data)
+
+
 def _token_stride(t: torch.Tensor, shape, name: str) -> int:
     """Elements between consecutive tokens of [n_seq, n_new, heads, head_dim],
     a slice of a fused projection or contiguous."""
@@ -153,18 +163,16 @@ class PagedStore:
                 return fn(*args, _raw_stream(self._index))
         return fn(*args, _raw_stream(self._index))
 
-    def _run(self, name: str, args: bytes, workspace: torch.Tensor | None):
+    def _run(self, fn, size, args: bytes, workspace: torch.Tensor | None):
         """A call with a workspace: the given one, or one of the size asked for."""
-        lib = _library()
-        fn = getattr(lib, name)
         if workspace is not None:
             if workspace.get_device() != self._index or not workspace.is_contiguous():
                 raise ValueError("workspace must be a contiguous tensor on the store's device")
-            rc = self._call(fn, args, workspace.data_ptr(), workspace.numel() * workspace.element_size())
+            rc = self._call(fn, args, workspace.data_ptr(), workspace.nbytes)
         else:
             rc = self._call(fn, args, None, 0)
             if rc == _capi.E_WORKSPACE:
-                n = getattr(lib, name + "_size")(args)
+                n = size(args)
                 workspace = torch.empty(n, dtype=torch.uint8, device=self.device)
                 rc = self._call(fn, args, workspace.data_ptr(), n)
         if rc:
@@ -256,14 +264,12 @@ class PagedStore:
             listed = pages.data_ptr()
         host = 0
         if seq_lens_host is not None:
-            seq_lens_host = np.ascontiguousarray(seq_lens_host, np.int32)
-            if seq_lens_host.size != self.n_seq:
-                raise ValueError("seq_lens_host must have one entry per sequence")
-            host = seq_lens_host.__array_interface__["data"][0]
+            host, seq_lens_host = _host_address(seq_lens_host, self.n_seq)
         args = self._store + _DECODE.pack(
             q.data_ptr(), out.data_ptr(), self._lens(seq_lens, "seq_lens"), self._lens(q_lens, "q_lens"), listed, n_select,
             shape[1], shape[2], num_splits, scale, self._dt16 if out.dtype is self.dtype else _dt(out.dtype), host)
-        self._run("gqa_decode_paged", args, workspace)
+        lib = _library()
+        self._run(lib.gqa_decode_paged, lib.gqa_decode_paged_size, args, workspace)
         return out
 
     def attention_workspace(self, q_len: int, n_heads: int, *, n_select: int = 0) -> torch.Tensor:
@@ -300,7 +306,8 @@ class PagedStore:
         args = self._store + _SELECT.pack(
             q.data_ptr(), out.data_ptr(), self._lens(seq_lens, "seq_lens"), self._lens(q_lens, "q_lens"), qs[1], qs[2],
             n_select, first, last)
-        self._run("page_select", args, workspace)
+        lib = _library()
+        self._run(lib.page_select, lib.page_select_size, args, workspace)
         return out
 
     # ------------------------------------------------------------- prefill
@@ -321,7 +328,8 @@ class PagedStore:
             self._like(out, shape, "out")
         args = self._store + _PREFILL.pack(q.data_ptr(), out.data_ptr(), seq, shape[0], start_pos, shape[1], scale,
                                            _dt(out.dtype))
-        self._run("gqa_prefill_paged", args, workspace)
+        lib = _library()
+        self._run(lib.gqa_prefill_paged, lib.gqa_prefill_paged_size, args, workspace)
         return out
 
     def prefill_workspace(self, n_tokens: int, n_heads: int, start_pos: int = 0) -> torch.Tensor:
@@ -373,6 +381,7 @@ class KVCachePaged:
         self.seq_lens_host = np.zeros(n_seq, np.int32)
         self._table = np.full((n_seq, per_seq), -1, np.int32)
         self._pages = np.zeros(n_seq, np.int64)  # held by each sequence
+        self._low = np.zeros(n_seq, np.int64)  # from there on each sequence's rows are in its ring (8-bit)
         self._free = list(range(n_pages - 1, -1, -1))
         self._pending = None  # the step's tokens per sequence (host)
 
@@ -396,27 +405,32 @@ class KVCachePaged:
 
     def release(self, seq: int) -> None:
         """Drop sequence `seq`: its pages are free again, its length is 0."""
+        if self._pending is not None:
+            raise RuntimeError("a step is under way: advance() first")
         held = int(self._pages[seq])
         self._free.extend(int(x) for x in self._table[seq, :held][::-1])
         self._table[seq, :] = -1
         self._pages[seq] = 0
         self.page_table[seq].fill_(-1)
+        self._low[seq] = 0
         self._set(seq, 0)
 
     def truncate(self, seq: int, tokens: int) -> None:
-        """Take back sequence `seq`'s newest tokens (rejected drafts); with 8-bit
-        pages at most ring - page_tokens of them."""
+        """Take back sequence `seq`'s newest tokens (rejected drafts).  With 8-bit
+        pages the rows of the page that is open then must still be in the ring
+        (always so for max_new tokens, and at a page's end)."""
+        if self._pending is not None:
+            raise RuntimeError("a step is under way: advance() first")
         held = int(self.seq_lens_host[seq])
         if not 0 <= tokens <= held:
             raise ValueError(f"{tokens} tokens of {held}")
-        s = self.layers[0]
-        if s.tail_k is not None and tokens and held - tokens > s.tail_k.shape[1] - self.page_tokens:
+        s, open_page = self.layers[0], tokens // self.page_tokens * self.page_tokens
+        if s.tail_k is not None and tokens != open_page and open_page < self._low[seq]:
             raise ValueError("the ring no longer holds that page's rows")
+        self._low[seq] = min(self._low[seq], tokens)
         self._set(seq, tokens)
 
     def _set(self, seq: int, tokens: int) -> None:
-        if self._pending is not None:
-            raise RuntimeError("a step is under way: advance() first")
         self.seq_lens_host = self.seq_lens_host.copy()  # (an earlier hint may still be read)
         self.seq_lens_host[seq] = tokens
         self.seq_lens[seq] = tokens
@@ -469,3 +483,5 @@ class KVCachePaged:
             return
         self.seq_lens.copy_(self._next)
         self.seq_lens_host, self._pending = self._after.astype(np.int32), None
+        if self.layers[0].tail_k is not None:
+            self._low = np.maximum(self._low, self.seq_lens_host - self.layers[0].tail_k.shape[1])

@@ -188,6 +188,30 @@ def test_drafts_taken_back(device):
     assert torch.equal(s.tail_k[:, 32:36], r.tail_k[:, 32:36])
 
 
+def test_how_far_a_sequence_goes_back(device):
+    """KVCachePaged.truncate: as far as the ring still holds the open page's rows, counted
+    from the longest the sequence has been; a page's end needs none."""
+    kv = mugen_amd.KVCachePaged(1, 1, 1, 64, 512, page_tokens=32, max_new=32, device=device)  # ring 64
+    k = P.randn(37, 1, 200, 1, 64)
+    kv.append(0, k, k)
+    with pytest.raises(RuntimeError):
+        kv.truncate(0, 100)
+    with pytest.raises(RuntimeError):
+        kv.release(0)
+    kv.advance()
+    kv.truncate(0, 170)  # open page 160: the ring holds 136 .. 199
+    with pytest.raises(ValueError):
+        kv.truncate(0, 150)  # open page 128
+    kv.truncate(0, 128)
+    kv.append(0, k[:, :7].contiguous(), k[:, :7].contiguous())
+    kv.advance()
+    with pytest.raises(ValueError):
+        kv.truncate(0, 140)  # longer than it is
+    kv.truncate(0, 130)  # its open page 128 is behind the ring of 200, but was written again ...
+    kv.release(0)
+    assert kv.free_pages == 16 and kv.seq_lens.tolist() == [0]
+
+
 @pytest.mark.parametrize("bits", [16, 8])
 def test_dropped_rows(device, bits):
     """Past max_seq_len, and in pages that are not there: nothing is written."""

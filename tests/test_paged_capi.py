@@ -135,7 +135,7 @@ def test_append_of_nothing():
 
 
 @pytest.mark.parametrize("kw,code", [
-    (dict(q=0), I), (dict(out=0), I), (dict(seq_lens=0), I), (dict(q=0x1008), I), (dict(q_len=0), U), (dict(q_len=65), U),
+    (dict(q=0), I), (dict(out=0), I), (dict(seq_lens=0), I), (dict(q=0x1008), I), (dict(out=0x1008), I), (dict(q_len=0), U), (dict(q_len=65), U),
     (dict(num_splits=-1), I), (dict(num_splits=129), I), (dict(out_dtype=7), U), (dict(pages=0x1000, n_select=0), I),
     (dict(scale=float("nan")), I), (dict(scale=float("inf")), I),
 ])
