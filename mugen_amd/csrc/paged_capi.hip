@@ -217,6 +217,35 @@ int64_t decode_items(const mugen_attn_gqa_decode_paged_args* a, int chunk, int64
     return n * each;
 }
 
+// Whether one split a range (no partials, no merge launch) is as fast as the cut into
+// `chunk`: a model in us of what was measured, kernel and merge, in captured steps.  A
+// workgroup takes 128 tokens in `step` us while it waits for nothing but its own
+// chain, all together stream at most 4.8 TB/s, and the two overlap by half; ragged
+// ranges end in a tail of the longest; the merge costs its launch and the partials'
+// way.  (28 / 4 heads d128, 8-bit, us
+// unsplit / cut: 1 x 512 7.7 / 7.4, 1 x 1024 10.4 / 7.5, 32 x 512 9.3 / 12.8, 32 x 1024 13.0
+// / 15.7; 16-bit 1 x 256 7.1 / 7.4, 8 x 384 9.1 / 8.1, 32 x 512 11.9 / 13.8; 32 / 8 d64 8-bit
+// 32 x 1024 10.9 / 14.0; 16 / 8 d256 8-bit 8 x 256 8.7 / 9.0, 8 x 768 15.9 / 13.6)
+bool one_split_pays(const mugen_attn_gqa_decode_paged_args* a, int wr, int nrb, int64_t len, int chunk) {
+    const mugen_attn_kv_pages& s = a->store;
+    const bool b8 = s.page_bits == 8;
+    const double step = (s.head_dim == 64 ? (b8 ? 0.5 : 0.7) : s.head_dim == 128 ? (b8 ? 0.65 : 1.7) : b8 ? 1.45 : 3.6) *
+                        (wr == 1 || wr == 3 ? 1.0 : wr == 2 ? 1.6 : 3.0);
+    double sum = 0;
+    for (int b = 0; b < s.n_seq; b++) sum += (double)range_len(a, b);
+    const double tail = 0.25 * ((double)len - sum / s.n_seq) / 128 * step;
+    if (a->pages) sum *= a->q_len;
+    constexpr double kRate = 4.8e6;  // bytes a us
+    const double stream = sum * s.n_kv_heads * nrb * 2 * s.head_dim * s.page_bits / 8 / kRate;
+    const double splits = (double)ceil_div(len, chunk);
+    const double partials = (double)s.n_seq * a->q_len * a->n_heads * splits * s.head_dim * 8 / kRate;
+    auto time = [&](int64_t tokens) {
+        const double chain = (double)tokens / 128 * step;
+        return std::max(chain, stream) + 0.5 * std::min(chain, stream);
+    };
+    return time(len) + tail <= time(chunk) + 2.6 + partials;
+}
+
 size_t decode_bytes(const mugen_attn_gqa_decode_paged_args* a, int splits) {
     if (splits <= 1) return 0;
     const size_t rows = (size_t)a->store.n_seq * a->q_len * a->n_heads;
@@ -247,9 +276,10 @@ DecodePlan decode_plan(const mugen_attn_gqa_decode_paged_args* a, bool for_size)
             else lo = mid + 32;
         }
         r.chunk = (int)hi;
+        if ((a->seq_lens_host || a->pages) && r.chunk < most && one_split_pays(a, r.wr, r.nrb, len, r.chunk)) r.chunk = (int)most;
         // large ragged batches: even items of 1024 tokens over several rounds, where
         // the longest range would run on alone
-        if (a->seq_lens_host && r.chunk > 1024) {
+        else if (a->seq_lens_host && r.chunk > 1024) {
             int64_t sum = 0;
             for (int b = 0; b < s.n_seq; b++) sum += range_len(a, b) * (a->pages ? a->q_len : 1);
             if ((double)std::min<int64_t>(r.chunk, len) * r.budget > 1.35 * (double)(sum * mult))

@@ -198,3 +198,27 @@ def test_a_workspace_asked_for_without_lengths_covers_every_copy(q_len, pages, h
                 host = np.ascontiguousarray(lens, dtype=np.int32)
                 a.seq_lens_host = host.ctypes.data
                 assert L.mugen_attn_gqa_decode_paged_workspace_size(ctypes.byref(a)) <= bound
+
+
+def splits(lens, H=28, Hk=4, D=128, bits=8, q_len=1, n_select=0, cache=16384):
+    """The plan's splits, from its workspace size (0: one, no partials)."""
+    host = np.ascontiguousarray(lens, np.int32)
+    a = make(_capi.GqaDecodePagedArgs, q_len=q_len, n_heads=H, s_n_seq=len(host), s_n_kv_heads=Hk, s_head_dim=D, s_page_bits=bits,
+             s_max_seq_len=cache, s_table_stride=cache // 64, s_tail_seq_stride=128 * Hk * D)
+    a.seq_lens_host = host.ctypes.data
+    if n_select:
+        a.pages, a.n_select = 0x1000, n_select
+    size = _capi.lib().mugen_attn_gqa_decode_paged_workspace_size(ctypes.byref(a))
+    return (size - 512) // (len(host) * q_len * H * (4 * D + 8)) if size else 1
+
+
+# short ranges, and batches that fill the card, are not cut; few long ones are
+@pytest.mark.parametrize("kw,whole", [
+    (dict(lens=[256]), True), (dict(lens=[512]), True), (dict(lens=[1024]), False), (dict(lens=[256], bits=16), True),
+    (dict(lens=[384], bits=16), False), (dict(lens=[1024] * 32), True), (dict(lens=[4096] * 8), False),
+    (dict(lens=[1024] * 32, H=32, Hk=8, D=64), True), (dict(lens=[256], H=16, Hk=8, D=256, bits=16), False),
+    (dict(lens=[9000] * 4, n_select=3), True), (dict(lens=[9000] * 4, n_select=64), False),
+    (dict(lens=[0]), True), (dict(lens=[1] * 200), True),
+])
+def test_plan_of_short_and_long_ranges(kw, whole):
+    assert (splits(**kw) == 1) == whole
