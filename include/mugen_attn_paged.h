@@ -192,8 +192,12 @@ int mugen_attn_page_select(const mugen_attn_page_select_args* args, void* worksp
 
 /*
  * Causal prefill of one sequence's chunk over the paged cache: the rules of
- * mugen_attn_gqa_prefill (BF16 V within +-65504), the keys being those the cache holds once the chunk is
- * appended (whole pages of an 8-bit store as their codes' values).
+ * mugen_attn_gqa_prefill (BF16 V within +-65504), the keys being those the cache
+ * holds once the chunk is appended (whole pages of an 8-bit store as their codes'
+ * values).  Chunks of few rows read the pages in place, longer ones from a copy
+ * in the workspace; every page_table entry up to start_pos + n_tokens has to be
+ * a page (one that is not is never followed, but counts as zero rows in the
+ * copy and as absent tokens in place).
  *   q, out   [n_tokens][n_heads][head_dim]; token i sees start_pos + i + 1 keys
  *   seq      the sequence: row of page_table and of the tail ring, which hold
  *            start_pos + n_tokens tokens

@@ -119,6 +119,12 @@ extern "C" int mugen_attn_kv_paged_append(const mugen_attn_kv_paged_append_args*
     const mugen_attn_kv_pages& s = a->store;
     if (int rc = store_validate(s, who)) return rc;
     if (a->n_new < 0) return fail(MUGEN_ATTN_E_INVALID, "%s: n_new < 0", who);
+    if (a->rope_dim < 0 || a->rope_dim > s.head_dim || a->rope_dim % 16)
+        return fail(MUGEN_ATTN_E_UNSUPPORTED, "%s: rope_dim %d (supported: multiples of 16 up to head_dim)", who, a->rope_dim);
+    const mugen_attn_rope_params& r = a->rope;
+    if (a->rope_dim && (!std::isfinite(r.theta) || !(r.theta > 0.f) || !std::isfinite(r.factor) ||
+                        (r.factor > 1.f && (r.original_ctx <= 0 || !(r.theta > 1.f)))))
+        return fail(MUGEN_ATTN_E_INVALID, "%s: bad rope parameters", who);
     if (a->n_new == 0 && !a->seq_lens_out) return MUGEN_ATTN_OK;
     if (!a->seq_lens) return fail(MUGEN_ATTN_E_INVALID, "%s: null seq_lens", who);
     if (a->seq_lens_out == a->seq_lens) return fail(MUGEN_ATTN_E_INVALID, "%s: seq_lens_out aliases seq_lens", who);
@@ -136,12 +142,6 @@ extern "C" int mugen_attn_kv_paged_append(const mugen_attn_kv_paged_append_args*
         if (!aligned16(a->q) || !aligned16(a->q_out) || a->q_stride % 8 || a->q_stride < (int64_t)a->n_heads * s.head_dim)
             return fail(MUGEN_ATTN_E_INVALID, "%s: q / q_out must be 16-byte aligned, q_stride a multiple of 8 and a row", who);
     }
-    if (a->rope_dim < 0 || a->rope_dim > s.head_dim || a->rope_dim % 16)
-        return fail(MUGEN_ATTN_E_UNSUPPORTED, "%s: rope_dim %d (supported: multiples of 16 up to head_dim)", who, a->rope_dim);
-    const mugen_attn_rope_params& r = a->rope;
-    if (a->rope_dim && (!std::isfinite(r.theta) || !(r.theta > 0.f) || !std::isfinite(r.factor) ||
-                        (r.factor > 1.f && (r.original_ctx <= 0 || !(r.theta > 1.f)))))
-        return fail(MUGEN_ATTN_E_INVALID, "%s: bad rope parameters", who);
     PagedAppendParams p{};
     p.st = store_params(s);
     p.k_new = static_cast<const uint16_t*>(a->k_new);

@@ -132,6 +132,8 @@ def test_append_refusals(kw, code):
 
 def test_append_of_nothing():
     assert call(make(_capi.KvPagedAppendArgs, n_new=0)) == _capi.OK
+    # a call without tokens checks the store and the rotation all the same
+    assert call(make(_capi.KvPagedAppendArgs, n_new=0, rope_dim=136)) == U
 
 
 @pytest.mark.parametrize("kw,code", [
