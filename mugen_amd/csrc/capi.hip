@@ -800,7 +800,8 @@ static PrefillSplit prefill_split_plan(const mugen_attn_gqa_prefill_args* a, int
     return r;
 }
 
-static PrefillSplit gqa_prefill_split(const mugen_attn_gqa_prefill_args* a) {
+// part32: fp32 partials at head_dim 64 and 128 too
+static PrefillSplit gqa_prefill_split(const mugen_attn_gqa_prefill_args* a, bool part32 = false) {
     PrefillSplit r;
     if (a->n_tokens <= 0 || a->kv_len <= 0) return r;
     if (a->head_dim > 128) {
@@ -838,7 +839,7 @@ static PrefillSplit gqa_prefill_split(const mugen_attn_gqa_prefill_args* a) {
     // ranges of at least 256 keys (4 steps of 64, 8 of 32): verify-sized
     // chunks (5 tokens after 4000, 7B shape) 18.1 -> 13.8 us against 512
     // keys; 4-head blocks at 128 keys measured slower (9.2 -> 10.3 us)
-    return prefill_split_plan(a, units, target, step, (size_t)a->head_dim * 2);
+    return prefill_split_plan(a, units, target, step, (size_t)a->head_dim * (part32 ? 4 : 2));
 }
 
 // The fp16 copy of V (one extra launch over kv_len rows): for long BF16
@@ -869,11 +870,11 @@ namespace mugen_attn {
 
 bool prefill_takes_v16(const mugen_attn_gqa_prefill_args* a) { return gqa_prefill_uses_v16(a) && !gqa_prefill_short_default(a); }
 
-size_t prefill_split_workspace(const mugen_attn_gqa_prefill_args* a) { return gqa_prefill_split(a).bytes; }
+size_t prefill_split_workspace(const mugen_attn_gqa_prefill_args* a) { return gqa_prefill_split(a, true).bytes; }
 
 // v16: a->v already is the fp16 copy (prefill_takes_v16), the workspace the
 // split partials' alone
-int prefill_run(const mugen_attn_gqa_prefill_args* a, bool v16, void* stream) {
+int prefill_run(const mugen_attn_gqa_prefill_args* a, bool v16, void* stream, bool part32) {
     if (int rc = gqa_prefill_validate(a)) return rc;
     if (a->n_tokens == 0) return MUGEN_ATTN_OK;
     GqaPrefillParams p{};
@@ -947,13 +948,14 @@ int prefill_run(const mugen_attn_gqa_prefill_args* a, bool v16, void* stream) {
     if (a->kernel) kernel = a->kernel;
     int dt = v16 ? kDtBf16V16 : a->dtype;
     const size_t v16_bytes = gqa_prefill_uses_v16(a) && !v16 ? gqa_prefill_ws(a) : 0;
-    const PrefillSplit split = gqa_prefill_split(a);  // none for the short kernel (default or forced)
+    const PrefillSplit split = gqa_prefill_split(a, part32);  // none for the short kernel (default or forced)
     p.ksplit = 1;
     if (split.ksplit > 1 && a->workspace && a->workspace_bytes >= v16_bytes + split.bytes) {
         // key splits (the warp-specialised kernel): partials after the V copy
         kernel = MUGEN_ATTN_PREFILL_KERNEL_WS;
         p.ksplit = split.ksplit;
         p.kchunk = split.kchunk;
+        p.part32 = part32;
         p.ws_ml = align256(static_cast<char*>(a->workspace) + v16_bytes);
         p.ws_o = reinterpret_cast<uint16_t*>(p.ws_ml + prefill_partials_at((size_t)a->n_tokens * a->n_heads * split.ksplit));
     }

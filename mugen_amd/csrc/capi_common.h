@@ -14,8 +14,9 @@ int hip_status(hipError_t e, const char* what);
 KernelTimer* active_timer();
 
 // mugen_attn_gqa_prefill, and the same for a caller that has V in fp16 already:
-// whether the call would copy it (BF16), and the workspace it then needs
-int prefill_run(const mugen_attn_gqa_prefill_args* a, bool v16, void* stream);
+// whether the call would copy it (BF16), and the workspace it then needs with the
+// key splits' partials in fp32 (part32)
+int prefill_run(const mugen_attn_gqa_prefill_args* a, bool v16, void* stream, bool part32 = false);
 bool prefill_takes_v16(const mugen_attn_gqa_prefill_args* a);
 size_t prefill_split_workspace(const mugen_attn_gqa_prefill_args* a);
 

@@ -866,15 +866,19 @@ __global__ __launch_bounds__(64 * (NS / SMB + NPV)) void gqa_prefill_ws_kernel(G
                 const float inv = linv_x[hb + hh][n];
                 if (SPLIT) {
                     // split partial: O / l in fp16 (a convex combination of
-                    // V rows, inside V's +-65504); l and the max from the S waves
+                    // V rows, inside V's +-65504) or, where asked for
+                    // (OUT_DT), fp32; l and the max from the S waves
                     const int64_t row = (int64_t)tok * p.H + kvh * G + NS * slice + hb + hh;
-                    uint16_t* dst = p.ws_o + (row * p.ksplit + ks_id) * hd + 4 * g;
+                    const int64_t at = (row * p.ksplit + ks_id) * hd + 4 * g;
 #pragma unroll
                     for (int d = 0; d < DB; d++) {
                         if (16 * d + 4 * g >= hd) break;  // padded dims (head_dim < D)
                         const f32x4_t r = o[hh][d] * inv;
-                        *reinterpret_cast<u32x2_t*>(dst + 16 * d) =
-                            u32x2_t{pack2<DT_F16>(r[0], r[1]), pack2<DT_F16>(r[2], r[3])};
+                        if constexpr (OUT_DT == DT_F32)
+                            *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(p.ws_o) + at + 16 * d) = r;
+                        else
+                            *reinterpret_cast<u32x2_t*>(p.ws_o + at + 16 * d) =
+                                u32x2_t{pack2<DT_F16>(r[0], r[1]), pack2<DT_F16>(r[2], r[3])};
                     }
                     continue;
                 }
@@ -1236,7 +1240,8 @@ constexpr int kWsTps = DT == DT_BF16 ? 1 : 2;
 // (token, head); with o_s = O_s / l_s stored, out = sum_s w_s o_s / sum_s w_s,
 // w_s = 2^(m_s - M) l_s, M the largest reference max (a split that saw no
 // key of the row: m = -inf, l = 0, weight 0)
-// PDT: the partials' type, fp16 (head_dim up to 128) or fp32 (above).
+// PDT: the partials' type, fp16 (head_dim up to 128) or fp32 (above, and over a
+// paged cache).
 template <int OUT_DT, int MAXS, int PDT>
 __global__ __launch_bounds__(256) void gqa_prefill_combine_kernel(GqaPrefillParams p) {
     using part_t = std::conditional_t<PDT == DT_F32, f32x4_t, u32x2_t>;
@@ -1315,8 +1320,8 @@ int gqa_prefill_ws_step_keys(int G, int dt) { return (G <= 4 || dt == DT_BF16) ?
 // two at head_dim 128, three at 64
 int gqa_prefill_ws_blocks_per_cu(int G, int D) { return G > 4 ? 1 : (D > 64 ? 2 : 3); }
 
-// SPLIT: the kernel stores fp16 partials whatever the output type (one
-// instantiation, OUT_DT = f32), and the combine writes the output
+// SPLIT: the kernel stores partials of type OUT_DT, fp16 or f32, whatever the
+// output type, and the combine writes the output
 template <int D, bool PAD, int DT, int OUT_DT, bool SPLIT>
 static hipError_t launch_pf_ws_k(const GqaPrefillParams& p, int Hk, hipStream_t st, KernelTimer* t) {
     const int nqb = (p.N + 15) / 16;
@@ -1341,7 +1346,12 @@ template <int D, bool PAD, int DT, int OUT_DT>
 static hipError_t launch_pf_ws_t(const GqaPrefillParams& p, int Hk, hipStream_t st, KernelTimer* t) {
     if (p.ksplit <= 1) return launch_pf_ws_k<D, PAD, DT, OUT_DT, false>(p, Hk, st, t);
     if (p.ksplit > kPrefillMaxSplits) return hipErrorInvalidValue;  // the merge's unrolled bound
-    const hipError_t e = launch_pf_ws_k<D, PAD, DT, DT_F32, true>(p, Hk, st, t);
+    if constexpr (!PAD)
+        if (p.part32) {
+            const hipError_t e = launch_pf_ws_k<D, PAD, DT, DT_F32, true>(p, Hk, st, t);
+            return e != hipSuccess ? e : launch_pf_combine<OUT_DT, DT_F32>(p, st, t);
+        }
+    const hipError_t e = launch_pf_ws_k<D, PAD, DT, DT_F16, true>(p, Hk, st, t);
     return e != hipSuccess ? e : launch_pf_combine<OUT_DT, DT_F16>(p, st, t);
 }
 

@@ -119,13 +119,14 @@ struct GqaPrefillParams {
     int hd;          // head_dim of q, the caches and out (<= D, a multiple of 8)
     // key splits (warp-specialised kernel; 1 = none): workgroup split s takes
     // keys [s kchunk, (s+1) kchunk) of its query block and writes the rows'
-    // normalised partial O (O_s / l_s, fp16; fp32 above head_dim 128, where
-    // ws_o points to floats) to ws_o [N][H][ksplit][hd] and
+    // normalised partial O (O_s / l_s, fp16; fp32 above head_dim 128 and with
+    // part32 (head_dim 64 and 128), where ws_o points to floats) to ws_o [N][H][ksplit][hd] and
     // (reference max in log2 units, weight sum l_s) to ws_ml
     // [N][H][ksplit][2]; the gqa_prefill_combine kernel then merges them
     // into out
     int ksplit;
     int kchunk;
+    int part32;
     uint16_t* ws_o;
     float* ws_ml;
 };

@@ -559,5 +559,5 @@ extern "C" int mugen_attn_gqa_prefill_paged(const mugen_attn_gqa_prefill_paged_a
         g.workspace = base + 2 * gather_bytes(a);
         g.workspace_bytes = more;
     }
-    return prefill_run(&g, p.v16, stream);
+    return prefill_run(&g, p.v16, stream, true);
 }

@@ -216,3 +216,22 @@ def test_prefill(device, bits, H, Hk, D, page, n, start):
             # (the prompt kernels weight bf16 V in fp16 too)
             want, tol = P.attend(q[i].cpu(), K[1][:start + i + 1], V[1][:start + i + 1], tol_dtype=F16)
             P.check(out[i], want, tol * 2, dtype, f"token {i}")
+
+
+@pytest.mark.parametrize("H,Hk,D,n,start", [(28, 4, 128, 100, 3000), (32, 8, 64, 80, 2500)])
+def test_prefill_split_partials_keep_small_values(device, H, Hk, D, n, start):
+    """Key ranges that are merged keep 32 bits: V of 1 .. 4 times the least
+    fp16 number, whose means fp16 cannot hold."""
+    P.say(f"prefill of least values H={H}/{Hk} D={D} n={n} start={start}")
+    T = start + n
+    store, K, _ = P.make_store(93, [40, T], Hk, D, 64, 16, F16, junk=False)
+    g = torch.Generator().manual_seed(94)
+    v = torch.randint(1, 5, store.v_pages.shape, generator=g).to(torch.float64) * 2.0 ** -24
+    store.v_pages.copy_(v.to(F16))
+    pages = store.page_table[1, :-(-T // 64)].long().cpu()
+    V = v[pages].transpose(1, 2).reshape(-1, Hk, D)[:T]
+    q = P.randn(95, n, H, D)
+    out = store.prefill(q, 1, start, out_dtype=torch.float32).cpu()
+    for i in (0, n // 2, n - 1):
+        want, tol = P.attend(q[i].cpu(), K[1][:start + i + 1], V[:start + i + 1], tol_dtype=F16)
+        P.check(out[i], want, tol, torch.float32, f"token {i}")
