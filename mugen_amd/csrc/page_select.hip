@@ -9,7 +9,10 @@
 // any order but for terms 2^30 apart, and a page next to the border does not change
 // sides with the kernel's tiling.  16 lanes take a page (2 * head_dim contiguous values), 4 pages
 // a wave instruction; every query of a sequence is scored from one read.
-// Bound: HBM (4 * head_dim bytes a page and kv head).
+// Bound: HBM (4 * head_dim bytes a page and kv head) past some ten MB, latency below:
+// the launch and four dependent reads (lengths, table, ranges, queries).  4.2 MB of
+// one sequence of 131k tokens 4.3 us, 17.7 MB of 16 sequences 8.7 (2 TB/s).  (The
+// queries' loads ahead of the table's: no gain, 4.3 and 9.0.)
 //
 // Choice.  Scores become 64-bit integers of the same order, held in registers.  One
 // histogram over 1024 equal bins between the least and the largest score finds the bin
@@ -18,7 +21,8 @@
 // pass from the highest bit in which any two candidates differ, then, among equal
 // keys, over the page number (the lowest pages win).  Either way the choice is a
 // border (key, page), and a ballot with one scan places the ascending list.
-// Bound: latency, a chain of 8 barriers (radix passes alone: 20; 2048 pages 7.7 us).
+// Bound: latency, a chain of 8 barriers (radix passes alone: 20, 2048 pages 7.7 us;
+// now 5.8, and 4.7 to 5.6 up to 1024 pages).
 #include <algorithm>
 
 #include "paged.h"
