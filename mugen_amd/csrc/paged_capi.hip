@@ -167,7 +167,8 @@ extern "C" int mugen_attn_kv_paged_append(const mugen_attn_kv_paged_append_args*
     p.heads_per_thread = (int)std::min<int64_t>(8, std::max<int64_t>(1, tokens * heads * (s.head_dim / 16) / (64 * 1024)));
     p.pages = (a->n_new + s.page_tokens - 1) / s.page_tokens;  // that n_new tokens can fill
     const int64_t jobs = (int64_t)s.n_seq * p.pages * s.n_kv_heads * 2;
-    if (tokens * heads * (s.head_dim / 16) > INT32_MAX || jobs > INT32_MAX / 2)
+    // (a launch takes less than 2^32 threads: 2^24 workgroups, at most half of them rows)
+    if (tokens * heads * (s.head_dim / 16) > INT32_MAX || jobs >= 1 << 23)
         return fail(MUGEN_ATTN_E_UNSUPPORTED, "%s: too many tokens in one call", who);
     return hip_status(launch_paged_append(p, turns, s.head_dim, s.dtype, s.page_bits == 8, static_cast<hipStream_t>(stream),
                                           active_timer()),
@@ -361,8 +362,9 @@ int decode_run(const mugen_attn_gqa_decode_paged_args* a, const DecodePlan& plan
         p.ws_ml = p.ws_o + slots * s.head_dim;
         p.plan = reinterpret_cast<int*>(p.ws_ml + slots * 2);
     }
-    // (work items are counted in 23 bits, the merge's grid in 16)
-    if (plan.nwg >= 1 << 23 || (int64_t)s.n_seq * (s.head_dim / 64) > 65535)
+    // (work items are counted in 23 bits, their launch, of up to 768 threads each, takes
+    // less than 2^32; the merge's grid in 16 bits)
+    if (plan.nwg >= 1 << 22 || (int64_t)s.n_seq * (s.head_dim / 64) > 65535)
         return fail(MUGEN_ATTN_E_UNSUPPORTED, "gqa_decode_paged: too many sequences or work items");
     hipError_t e = s.page_bits == 8
                        ? launch_paged_decode8(p, (int)plan.nwg, s.head_dim, s.dtype, plan.wr, st, active_timer())

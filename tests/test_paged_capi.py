@@ -130,6 +130,14 @@ def test_append_refusals(kw, code):
     assert call(make(_capi.KvPagedAppendArgs, **kw)) == code
 
 
+def test_refusals_of_too_large_launches():
+    """2^32 threads and more: 134 million page jobs, 5 million work items of 768 threads."""
+    big = dict(s_n_seq=65535, s_n_kv_heads=1024, s_tail_seq_stride=128 * 1024 * 128)
+    assert call(make(_capi.KvPagedAppendArgs, n_new=1, q=0, k_stride=1024 * 128, v_stride=1024 * 128, **big)) == U
+    big = dict(s_n_seq=5000, s_n_kv_heads=1000, s_tail_seq_stride=128 * 1000 * 128)
+    assert call(make(_capi.GqaDecodePagedArgs, n_heads=16000, q_len=3, **big), 0x1000, 1 << 60) == U
+
+
 def test_append_of_nothing():
     assert call(make(_capi.KvPagedAppendArgs, n_new=0)) == _capi.OK
     # a call without tokens checks the store and the rotation all the same
