@@ -216,7 +216,7 @@ class PagedStore:
             raise ValueError("k_new and v_new must be [n_seq, n_new, n_kv_heads, head_dim]")
         n_new = shape[1]
         if n_new == 0:
-            return q_out
+            raise ValueError("append needs a token (new_lens may leave sequences without)")
         qp = qo = q_stride = H = 0
         if q is not None:
             qs = self._heads(q, "q")
@@ -260,6 +260,8 @@ class PagedStore:
         listed = n_select = 0
         if pages is not None:
             n_select = pages.shape[-1]
+            if n_select == 0:
+                raise ValueError("pages must list at least one entry")
             self._like(pages, (*shape[:2], self.n_kv_heads, n_select), "pages", _i32)
             listed = pages.data_ptr()
         host = 0
@@ -444,7 +446,8 @@ class KVCachePaged:
         counts = np.full(self.n_seq, n_new, np.int32) if new_lens is None else np.asarray(new_lens, np.int32)
         if counts.shape != (self.n_seq,) or (counts < 0).any() or (counts > n_new).any():
             raise ValueError("new_lens must be [n_seq], each 0 .. n_new")
-        if self._pending is None:
+        first = self._pending is None
+        if first:
             after = self.seq_lens_host + counts
             if (after > self.max_seq_len).any():
                 raise RuntimeError("a sequence would pass max_seq_len")
@@ -454,8 +457,13 @@ class KVCachePaged:
             self._pending, self._after = counts, after
         elif not np.array_equal(self._pending, counts):
             raise ValueError("every layer of a step appends the same tokens")
-        return self.layers[layer].append(k_new, v_new, self.seq_lens, new_lens=self._new, seq_lens_out=self._next, q=q,
-                                         rope=rope, rope_dim=rope_dim)
+        try:
+            return self.layers[layer].append(k_new, v_new, self.seq_lens, new_lens=self._new, seq_lens_out=self._next, q=q,
+                                             rope=rope, rope_dim=rope_dim)
+        except Exception:
+            if first:  # no step is under way: its lengths were not written
+                self._pending = None
+            raise
 
     def _now(self):
         """Lengths with the step's tokens, and how many each sequence has."""

@@ -403,3 +403,27 @@ def test_another_stream(device):
         got = s.attention(q2, i32([300, 40]))
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_a_refused_append_starts_no_step(device):
+    """A first append that is refused leaves the lengths alone: advance() has nothing to commit;
+    no step is without tokens, and no page list without entries."""
+    kv = mugen_amd.KVCachePaged(1, 2, 1, 64, 256, page_tokens=32, max_new=32, device=device)
+    k = P.randn(38, 2, 5, 1, 64)
+    kv.append(0, k, k)
+    kv.advance()
+    for bad in (k.to(BF16), k[:, :3], k[..., :32].contiguous()):
+        with pytest.raises(ValueError):
+            kv.append(0, k, bad)
+        kv.advance()
+        assert kv.seq_lens.tolist() == [5, 5] and kv.seq_lens_host.tolist() == [5, 5]
+    with pytest.raises(ValueError):
+        kv.append(0, k[:, :0], k[:, :0])
+    s = kv.layers[0]
+    with pytest.raises(ValueError):
+        s.append(k[:, :0], k[:, :0], kv.seq_lens, seq_lens_out=torch.zeros_like(kv.seq_lens))
+    with pytest.raises(ValueError):
+        s.attention(k[:, :1].contiguous(), kv.seq_lens, pages=torch.zeros((2, 1, 1, 0), dtype=torch.int32, device=device))
+    kv.append(0, k, k)
+    kv.advance()
+    assert kv.seq_lens.tolist() == [10, 10]
