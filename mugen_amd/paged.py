@@ -212,8 +212,9 @@ class PagedStore:
         rotation; rope_dim: the rotated dims (default head_dim).  new_lens: tokens
         each sequence gets (default n_new); rows behind them are not touched."""
         shape = self._heads(k_new, "k_new")
-        if shape[2] != self.n_kv_heads or self._heads(v_new, "v_new") != shape:
-            raise ValueError("k_new and v_new must be [n_seq, n_new, n_kv_heads, head_dim]")
+        if shape[2] != self.n_kv_heads or v_new.shape != shape or v_new.dtype is not self.dtype or \
+                v_new.get_device() != self._index:
+            raise ValueError("k_new and v_new must be [n_seq, n_new, n_kv_heads, head_dim] in the store's dtype, on its device")
         n_new = shape[1]
         if n_new == 0:
             raise ValueError("append needs a token (new_lens may leave sequences without)")
@@ -226,13 +227,18 @@ class PagedStore:
                 q_out = torch.empty(qs, dtype=q.dtype, device=q.device)
             else:
                 self._like(q_out, qs, "q_out", self.dtype)
-            qp, qo, q_stride, H = q.data_ptr(), q_out.data_ptr(), _token_stride(q, qs, "q"), qs[2]
+            H = qs[2]
+            qp, qo = q.data_ptr(), q_out.data_ptr()
+            q_stride = H * self.head_dim if q.is_contiguous() else _token_stride(q, qs, "q")
+        row = self.n_kv_heads * self.head_dim
         theta, factor, ctx = (0.0, 0.0, 0) if rope is None else rope
         dim = 0 if rope is None else self.head_dim if rope_dim is None else int(rope_dim)
         args = self._store + _APPEND.pack(
-            k_new.data_ptr(), v_new.data_ptr(), qp, qo, self._lens(seq_lens, "seq_lens"), self._lens(new_lens, "new_lens"),
-            self._lens(seq_lens_out, "seq_lens_out"), _token_stride(k_new, shape, "k_new"),
-            _token_stride(v_new, shape, "v_new"), q_stride, n_new, H, dim, theta, factor, ctx)
+            k_new.data_ptr(), v_new.data_ptr(), qp, qo, self._lens(seq_lens, "seq_lens"),
+            0 if new_lens is None else self._lens(new_lens, "new_lens"),
+            0 if seq_lens_out is None else self._lens(seq_lens_out, "seq_lens_out"),
+            row if k_new.is_contiguous() else _token_stride(k_new, shape, "k_new"),
+            row if v_new.is_contiguous() else _token_stride(v_new, shape, "v_new"), q_stride, n_new, H, dim, theta, factor, ctx)
         rc = self._call(_library().append, args)
         if rc:
             _capi.check(rc)
@@ -268,7 +274,8 @@ class PagedStore:
         if seq_lens_host is not None:
             host, seq_lens_host = _host_address(seq_lens_host, self.n_seq)
         args = self._store + _DECODE.pack(
-            q.data_ptr(), out.data_ptr(), self._lens(seq_lens, "seq_lens"), self._lens(q_lens, "q_lens"), listed, n_select,
+            q.data_ptr(), out.data_ptr(), self._lens(seq_lens, "seq_lens"),
+            0 if q_lens is None else self._lens(q_lens, "q_lens"), listed, n_select,
             shape[1], shape[2], num_splits, scale, self._dt16 if out.dtype is self.dtype else _dt(out.dtype), host)
         lib = _library()
         self._run(lib.gqa_decode_paged, lib.gqa_decode_paged_size, args, workspace)
@@ -306,7 +313,8 @@ class PagedStore:
         else:
             self._like(out, shape, "out", _i32)
         args = self._store + _SELECT.pack(
-            q.data_ptr(), out.data_ptr(), self._lens(seq_lens, "seq_lens"), self._lens(q_lens, "q_lens"), qs[1], qs[2],
+            q.data_ptr(), out.data_ptr(), self._lens(seq_lens, "seq_lens"),
+            0 if q_lens is None else self._lens(q_lens, "q_lens"), qs[1], qs[2],
             n_select, first, last)
         lib = _library()
         self._run(lib.page_select, lib.page_select_size, args, workspace)
