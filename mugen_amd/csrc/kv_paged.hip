@@ -19,7 +19,8 @@
 // writes them once it holds the old rows.
 //
 // Bound: the launch and two dependent reads (length, page table) for a few tokens: one
-// token of 28 / 4 heads 3.1 us, of 64 sequences of 32 / 8 heads with 8-bit pages 4.2.
+// token of 28 / 4 heads 3.1 us, of 64 sequences of 32 / 8 heads with 8-bit pages 4.2,
+// and 1.6 more where one of them fills a page (one job's loads, reduction and codes).
 // A prompt moves each row once and reads K and V once more for the pages: 2047 tokens
 // of 28 / 4 heads, 40 MB, 12.6 us (3.2 TB/s): one wave of workgroups whose loads, sines
 // and stores follow one another.
@@ -148,9 +149,31 @@ __device__ __forceinline__ void append_rows(const PagedAppendParams& p, const Ro
     }
 }
 
-// keeps a NaN once met
-__device__ __forceinline__ float nan_min(float a, float b) { return (b < a || b != b) ? b : a; }
-__device__ __forceinline__ float nan_max(float a, float b) { return (b > a || b != b) ? b : a; }
+// Two 16-bit floats as unsigned numbers of the same order, `lo` from below and `hi`
+// from above, so that the least of either is the minimum and the maximum; a NaN is the
+// least of both.  Packed 16-bit integers: 12 instructions for a pair and its two minima.
+using u16x2_t = unsigned short __attribute__((ext_vector_type(2)));
+using s16x2_t = short __attribute__((ext_vector_type(2)));
+template <int DT>
+__device__ __forceinline__ void range_keys(uint32_t x, uint32_t& lo, uint32_t& hi) {
+    const u16x2_t v = __builtin_bit_cast(u16x2_t, x), one = {1, 1};
+    const u16x2_t inf = DT == DT_F16 ? u16x2_t{0x7c00, 0x7c00} : u16x2_t{0x7f80, 0x7f80};
+    const u16x2_t sign = __builtin_bit_cast(u16x2_t, __builtin_bit_cast(s16x2_t, v) >> 15);
+    const u16x2_t key = v ^ (sign | u16x2_t{0x8000, 0x8000});
+    const u16x2_t nan = __builtin_elementwise_min(__builtin_elementwise_sub_sat(v & u16x2_t{0x7fff, 0x7fff}, inf), one);
+    const u16x2_t keep = nan - one;  // (0 for a NaN, else all ones)
+    lo = __builtin_bit_cast(uint32_t, key & keep);
+    hi = __builtin_bit_cast(uint32_t, ~key & keep);
+}
+__device__ __forceinline__ uint32_t least2(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+// the floats again (is_hi: from a `hi`)
+__device__ __forceinline__ uint32_t range_values(uint32_t k, bool is_hi) {
+    const u16x2_t key = __builtin_bit_cast(u16x2_t, is_hi ? ~k : k);
+    const u16x2_t pos = __builtin_bit_cast(u16x2_t, __builtin_bit_cast(s16x2_t, key) >> 15);
+    return __builtin_bit_cast(uint32_t, key ^ (~pos | u16x2_t{0x8000, 0x8000}));
+}
 
 // the page that job `id` is about, where this call fills it
 template <int D, int P, int DT, bool BITS8>
@@ -290,54 +313,60 @@ __device__ __forceinline__ void append_page(const PagedAppendParams& p, const Ro
         }
     }
     if (!ranged) return;
-    // minimum and maximum of each dim: a thread's own rows, then over the
-    // threads of the same dims through LDS, the maxima after the minima
-    float lo[16], hi[16];
+    // minimum and maximum of each dim: a thread's own rows, then over the lanes of the same
+    // dims (each exchange leaves a lane half of the words: the minima or the maxima, then
+    // the first or the second eight dims), then over the waves through LDS: 0.8 us of a step
+    // in which a page of 64 fills (all threads' values through LDS, twice: 2.6)
+    uint32_t m[16];
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-        lo[e] = -kNegInf;
-        hi[e] = kNegInf;
-    }
+    for (int e = 0; e < 16; e++) m[e] = 0xffffffffu;
     const float scale = exp_scale((uint32_t)byte);
 #pragma unroll
     for (int i = 0; i < UPT; i++) {
         if (threadIdx.x + 256 * i >= UNITS) continue;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            uint32_t w;
+            uint32_t w, lo, hi;
             if constexpr (BITS8)
                 w = (e & 1) ? cvt2_fp8<DT, true>(code[i][e >> 1], scale) : cvt2_fp8<DT, false>(code[i][e >> 1], scale);
             else w = e < 4 ? xa[i][e] : xb[i][e - 4];
-            const float x0 = lo_f32<DT>(w), x1 = hi_f32<DT>(w);
-            lo[2 * e] = nan_min(lo[2 * e], x0);
-            hi[2 * e] = nan_max(hi[2 * e], x0);
-            lo[2 * e + 1] = nan_min(lo[2 * e + 1], x1);
-            hi[2 * e + 1] = nan_max(hi[2 * e + 1], x1);
+            range_keys<DT>(w, lo, hi);
+            m[e] = least2(m[e], lo);
+            m[8 + e] = least2(m[8 + e], hi);
         }
     }
-    float* part = reinterpret_cast<float*>(lds);  // [256][16 + 1]
-    constexpr int ROWS = 256 / U;                 // threads of the same dims
 #pragma unroll
-    for (int pass = 0; pass < 2; pass++) {
-        __syncthreads();
+    for (int e = 0; e < 8; e++) {
+        const auto r = __builtin_amdgcn_permlane32_swap(m[e], m[8 + e], false, false);
+        m[e] = least2(r[0], r[1]);
+    }
 #pragma unroll
-        for (int e = 0; e < 16; e++) part[threadIdx.x * 17 + e] = pass ? hi[e] : lo[e];
-        __syncthreads();
-        if (threadIdx.x < D) {
-            const int u = threadIdx.x / 16, e = threadIdx.x % 16;
-            float m = part[u * 17 + e];
-            for (int r = 1; r < (ROWS < P ? ROWS : P); r++) {
-                const float x = part[(r * U + u) * 17 + e];
-                m = pass ? nan_max(m, x) : nan_min(m, x);
-            }
-            int d0, d1;
-            unit_dims(u, p.rope_dim, d0, d1);
-            p.st.k_range[(ph * 2 + pass) * D + (e < 8 ? d0 + e : d1 + e - 8)] = from_f32<DT>(m);
+    for (int e = 0; e < 4; e++) {
+        const auto r = __builtin_amdgcn_permlane16_swap(m[e], m[4 + e], false, false);
+        m[e] = least2(r[0], r[1]);
+        if constexpr (U <= 8) m[e] = least2(m[e], __float_as_uint(dpp_xor<8>(__uint_as_float(m[e]))));
+        if constexpr (U <= 4) m[e] = least2(m[e], __float_as_uint(dpp_xor<4>(__uint_as_float(m[e]))));
+    }
+    u32x4_t* part = reinterpret_cast<u32x4_t*>(lds);  // [wave][minimum, maximum][d0, d1][U]
+    const int lane = threadIdx.x & 63, l16 = lane & 15;
+    if (l16 < U) part[(threadIdx.x >> 6) * 4 * U + (lane >> 4) * U + l16] = u32x4_t{m[0], m[1], m[2], m[3]};
+    __syncthreads();
+    if (threadIdx.x < 4 * U) {
+        const int u = threadIdx.x % U, which = threadIdx.x / U;
+        u32x4_t r = part[threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < 4; w++) {
+            const u32x4_t x = part[w * 4 * U + threadIdx.x];
+#pragma unroll
+            for (int e = 0; e < 4; e++) r[e] = least2(r[e], x[e]);
         }
+#pragma unroll
+        for (int e = 0; e < 4; e++) r[e] = range_values(r[e], which >= 2);
+        int d0, d1;
+        unit_dims(u, p.rope_dim, d0, d1);
+        *reinterpret_cast<u32x4_t*>(p.st.k_range + (ph * 2 + (which >> 1)) * D + ((which & 1) ? d1 : d0)) = r;
     }
 }
-
-constexpr int kPageLds = 256 * 17 * 4;  // the ranges' partials; at least a page's V codes (32 KiB) where those are wider
 
 template <int D, int DT, bool BITS8>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p, RopeTurns<D / 2> turns) {
@@ -345,7 +374,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p, 
         append_rows<D, DT, BITS8>(p, turns, blockIdx.x * 256u + threadIdx.x);
         return;
     }
-    __shared__ __attribute__((aligned(16))) char lds[kPageLds > 128 * D ? kPageLds : 128 * D];
+    // a page's V codes; the ranges' partials of 4 waves, at most 4 KiB
+    __shared__ __attribute__((aligned(16))) char lds[BITS8 ? 128 * D : 4096];
     const int id = (int)blockIdx.x - p.row_blocks;
     if (p.st.p_shift == 5) append_page<D, 32, DT, BITS8>(p, turns, id, lds);
     else if (p.st.p_shift == 6) append_page<D, 64, DT, BITS8>(p, turns, id, lds);
