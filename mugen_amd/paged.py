@@ -355,7 +355,9 @@ class KVCachePaged:
 
     A step: reserve() pages where they run out, append() each layer's K and V
     (and rotate its queries), attention() over them, advance() once.  seq_lens is
-    kept on the device and on the host."""
+    kept on the device and on the host, so a step's append is not for graph
+    capture (it is refused); a captured step calls the layers' PagedStore with
+    device lengths."""
 
     def __init__(self, n_layers: int, n_seq: int, n_kv_heads: int, head_dim: int, max_seq_len: int = 8192, *,
                  n_pages: int | None = None, page_tokens: int = 64, page_bits: int = 8,
@@ -456,6 +458,8 @@ class KVCachePaged:
             raise ValueError("new_lens must be [n_seq], each 0 .. n_new")
         first = self._pending is None
         if first:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a replay would not move the host's lengths: capture the layers' PagedStore calls")
             after = self.seq_lens_host + counts
             if (after > self.max_seq_len).any():
                 raise RuntimeError("a sequence would pass max_seq_len")
@@ -482,6 +486,8 @@ class KVCachePaged:
     def attention(self, layer: int, q: torch.Tensor, *, pages: torch.Tensor | None = None, **kw) -> torch.Tensor:
         """PagedStore.attention of the step's tokens (appended to this layer before)."""
         lens, host, new = self._now()
+        if torch.cuda.is_current_stream_capturing():  # (replays see other lengths: planned from the device's)
+            host = None
         return self.layers[layer].attention(q, lens, q_lens=new, pages=pages, seq_lens_host=host, **kw)
 
     def select_pages(self, layer: int, q: torch.Tensor, n_select: int, **kw) -> torch.Tensor:

@@ -427,3 +427,30 @@ def test_a_refused_append_starts_no_step(device):
     kv.append(0, k, k)
     kv.advance()
     assert kv.seq_lens.tolist() == [10, 10]
+
+
+def test_a_cache_under_capture(device):
+    """KVCachePaged: a step is not captured; attention captured alone follows the device's
+    lengths on every replay."""
+    kv = mugen_amd.KVCachePaged(1, 2, 2, 64, 1024, page_tokens=32, max_new=32, device=device)
+    q = P.randn(40, 2, 1, 4, 64)
+    x = P.randn(41, 2, 40, 2, 64)
+    kv.append(0, x, x)
+    kv.advance()
+    ws = kv.layers[0].attention_workspace(1, 4)
+    out = torch.zeros_like(q)
+    kv.attention(0, q, out=out, workspace=ws)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kv.attention(0, q, out=out, workspace=ws)
+        with pytest.raises(RuntimeError):
+            kv.append(0, x, x)
+    for s in range(3):
+        y = P.randn(42 + s, 2, 300, 2, 64)
+        kv.append(0, y, y, new_lens=[300, 7 + s])
+        kv.advance()
+        out.zero_()
+        g.replay()
+        want = kv.layers[0].attention(q, kv.seq_lens)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), f"replay {s}"
