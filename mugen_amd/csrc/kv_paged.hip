@@ -197,6 +197,8 @@ __device__ __forceinline__ void append_page(const PagedAppendParams& p, const Ro
     if (phys < 0 && !(BITS8 && c == 0)) return;  // (its ring slots are still this job's)
     const int64_t ph = (int64_t)phys * Hk + kvh;
     const bool ranged = !is_v && p.st.k_range;
+    // (+: a choice of two values, where the choice of the two members copies the struct to scratch)
+    uint16_t* const tail = is_v ? +p.st.tail_v : +p.st.tail_k;
     u32x4_t xa[UPT], xb[UPT];
     float amax = 0.f;
 #pragma unroll
@@ -216,8 +218,7 @@ __device__ __forceinline__ void append_page(const PagedAppendParams& p, const Ro
         } else {
             const uint16_t* src;
             if constexpr (BITS8)
-                src = (is_v ? p.st.tail_v : p.st.tail_k) + b * p.st.tail_stride +
-                      ((int64_t)(t & (p.st.ring - 1)) * Hk + kvh) * D;
+                src = tail + b * p.st.tail_stride + ((int64_t)(t & (p.st.ring - 1)) * Hk + kvh) * D;
             else src = reinterpret_cast<const uint16_t*>(p.st.k) + (ph * P + r) * D;
             xa[i] = load16(src + d0);
             xb[i] = load16(src + d1);
@@ -254,7 +255,7 @@ __device__ __forceinline__ void append_page(const PagedAppendParams& p, const Ro
                 const uint16_t* src = (is_v ? p.v_new + row * p.v_stride : p.k_new + row * p.k_stride) + (int64_t)kvh * D;
                 u32x4_t x = load16(src + d0), y = load16(src + d1);
                 if (!is_v && 16 * u < p.rope_dim) rotate8<DT>(turn8(turns, u, t), x, y);
-                uint16_t* dst = (is_v ? p.st.tail_v : p.st.tail_k) + b * p.st.tail_stride + ((int64_t)slot * Hk + kvh) * D;
+                uint16_t* dst = tail + b * p.st.tail_stride + ((int64_t)slot * Hk + kvh) * D;
                 *reinterpret_cast<u32x4_t*>(dst + d0) = x;
                 *reinterpret_cast<u32x4_t*>(dst + d1) = y;
             }
@@ -284,7 +285,7 @@ __device__ __forceinline__ void append_page(const PagedAppendParams& p, const Ro
                 uint32_t w = enc(lo_f32<DT>(x[k]), hi_f32<DT>(x[k]), 0u, std::false_type{});
                 code[i][e] = enc(lo_f32<DT>(x[k + 1]), hi_f32<DT>(x[k + 1]), w, std::true_type{});
             }
-        if (threadIdx.x == 0) (is_v ? p.st.v_exp : p.st.k_exp)[ph] = (uint8_t)byte;
+        if (threadIdx.x == 0) (is_v ? +p.st.v_exp : +p.st.k_exp)[ph] = (uint8_t)byte;
 #pragma unroll
         for (int i = 0; i < UPT; i++) {
             const int unit = threadIdx.x + 256 * i;
