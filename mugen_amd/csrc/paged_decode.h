@@ -35,7 +35,7 @@
 //    are checked for values that are not finite; where one is met, each token's
 //    rows get their own product with the later rows zeroed;
 //  Bound: HBM for a batch (64 sequences of 512..8191 tokens, 32 / 8 heads, 8-bit: 570 MB
-//  read, no byte twice, in 121 us, 4.7 TB/s of a copy's 5.2; MFMA busy a tenth of the
+//  read, no byte twice, in 114 us, 5.0 TB/s of a copy's 5.2; MFMA busy a tenth of the
 //  time); 5 tokens of 4 x 31k 129 MB of codes in 31 us, 4.1 TB/s,
 //  beside the softmax of 48 rows (MFMA busy 15%); one sequence of 4096 latency, 5.6 us for 8.4 MB: the launch, four
 //  dependent reads and the merge of the waves;
@@ -317,12 +317,17 @@ __global__ __launch_bounds__(64 * WR * paged_tiles(D, BITS8, WR))
             vq[x] = load16(vb + min(x * RPL + lane / (RB / 16), last) * stride + 8 * (lane % (RB / 16)));
     };
     char* stage = &lds[w * 32 * RB];
+    // (opaque in the open page's loop, where these offsets had better be formed again than
+    // held in registers over the main loop: 64 sequences of 512..8191 tokens 125.9 -> 114.8 us)
+    int st_lane = lane;
     auto st_off = [&](int x) {
-        const int row = x * RPL + lane / (RB / 16), c = lane % (RB / 16);
+        const int row = x * RPL + st_lane / (RB / 16), c = st_lane % (RB / 16);
         return row * RB + ((c ^ swz<D>(row)) * 16);
     };
-    const int tr = 8 * g + (n >> 2);
-    auto t_off = [&](int d) { return tr * RB + (((2 * d + ((n & 3) >> 1)) ^ swz<D>(tr)) * 16) + 8 * (n & 1); };
+    auto t_off = [&](int d) {
+        const int sn = st_lane & 15, tr = 8 * (st_lane >> 4) + (sn >> 2);
+        return tr * RB + (((2 * d + ((sn & 3) >> 1)) ^ swz<D>(tr)) * 16) + 8 * (sn & 1);
+    };
     auto wave_sync = [] {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -587,6 +592,7 @@ __global__ __launch_bounds__(64 * WR * paged_tiles(D, BITS8, WR))
             for (; tt < hi; tt += STEP) {
                 const int t0 = (whole << ps) + (tt & (P - 1));  // its first token
                 if (t0 >= T) break;
+                asm volatile("" : "+v"(st_lane));
                 const int64_t ring_at = b * p.st.tail_stride + ((int64_t)(t0 & (p.st.ring - 1)) * Hk + kvh) * D;
                 u32x4_t kq[2][KK], vq[VL];
                 load16_tile(p.st.tail_k + ring_at, p.st.tail_v + ring_at, Hk * D, min(31, T - 1 - t0), kq, vq);
