@@ -19,10 +19,10 @@
 // writes them once it holds the old rows.
 //
 // Bound: the launch and two dependent reads (length, page table) for a few tokens: one
-// token of 28 / 4 heads 3.1 us, of 64 sequences of 32 / 8 heads with 8-bit pages 4.2,
-// and 1.6 more where one of them fills a page (one job's loads, reduction and codes).
+// token of 28 / 4 heads 3.1 us, of 64 sequences of 32 / 8 heads with 8-bit pages 4.0,
+// and 1.5 more where one of them fills a page (one job's loads, reduction and codes).
 // A prompt moves each row once and reads K and V once more for the pages: 2047 tokens
-// of 28 / 4 heads, 40 MB, 11.9 us a call (3.4 TB/s): one wave of workgroups whose loads, sines
+// of 28 / 4 heads, 40 MB, 11.4 us a call (3.5 TB/s): one wave of workgroups whose loads, sines
 // and stores follow one another.
 // The least e with amax <= 448 * 2^e: amax = m 2^x, 0.5 <= m < 1, is
 // m * 2^(x-9) * 512, so e = x - 9 where m <= 448/512, else x - 8: no division.

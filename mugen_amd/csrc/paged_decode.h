@@ -35,7 +35,7 @@
 //    are checked for values that are not finite; where one is met, each token's
 //    rows get their own product with the later rows zeroed;
 //  Bound: HBM for a batch (64 sequences of 512..8191 tokens, 32 / 8 heads, 8-bit: 570 MB
-//  read, no byte twice, in 114 us, 5.0 TB/s of a copy's 5.2; MFMA busy a tenth of the
+//  read, no byte twice, in 111 us, 5.1 TB/s of a copy's 5.2; MFMA busy a tenth of the
 //  time); 5 tokens of 4 x 31k 129 MB of codes in 31 us, 4.1 TB/s,
 //  beside the softmax of 48 rows (MFMA busy 15%); one sequence of 4096 latency, 5.6 us for 8.4 MB: the launch, four
 //  dependent reads and the merge of the waves;
